@@ -3,12 +3,16 @@
 ``knn``, ``knn_graph``, ``radius``, ``radius_graph``, ``nearest`` and ``fps``
 are drop-ins for the functions of the same name in ``torch_cluster``;
 importing this package registers ``torch.ops.torch_cluster.knn`` / ``radius``
-/ ``nearest`` / ``fps``.
+/ ``nearest`` / ``fps``.  ``attention``, ``norm_rotate`` and ``lookup`` work on
+the features of the same rows.
 """
 from . import _native  # noqa: F401  (loads the native libraries or raises)
+from .attention import attention
 from .fps import fps
 from .knn import knn, knn_graph
+from .lookup import lookup
 from .nearest import nearest
+from .norm_rotate import norm_rotate
 from .radius import radius, radius_graph
 
 import torch as _torch
@@ -35,4 +39,5 @@ def get_search_strategy() -> str:
 
 
 __all__ = ["knn", "knn_graph", "radius", "radius_graph", "nearest", "fps",
+           "attention", "norm_rotate", "lookup",
            "set_search_strategy", "get_search_strategy", "__version__"]

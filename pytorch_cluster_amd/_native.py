@@ -1,7 +1,8 @@
 """Loads the native libraries of this package.
 
 * ``libpca_neighbors.so`` -- HIP kernels behind the C ABI declared in
-  ``include/pca_neighbors.h`` (bound with ctypes as :data:`capi`).
+  ``include/pca_neighbors.h`` and ``include/pca_features.h`` (bound with ctypes
+  as :data:`capi`).
 * ``_torch_ops.so`` -- registers ``torch.ops.torch_cluster.knn`` /
   ``radius`` / ``nearest`` / ``fps`` / ``cuda_version``, the operators the reference package loads from
   its per-operator shared objects (``torch_cluster/__init__.py:8-21``).
@@ -106,11 +107,67 @@ C_ABI = {
 }
 
 
+class AttentionArgs(ctypes.Structure):
+    """``pca_attention_args`` of include/pca_features.h."""
+    _fields_ = (
+        [(n, _vp) for n in ("q", "k", "v")]
+        + [(n, _i64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row",
+                               "v_head")]
+        + [(n, _vp) for n in ("spans_q", "spans_k", "pos_q", "pos_k", "slope")]
+        + [("axes", ctypes.c_int32), ("dtype", ctypes.c_int32), ("nq", _i64),
+           ("nk", _i64), ("hq", ctypes.c_int32), ("hk", ctypes.c_int32),
+           ("d", ctypes.c_int32), ("scale", ctypes.c_float),
+           ("cap", ctypes.c_float)])
+
+
+class NormRotateArgs(ctypes.Structure):
+    """``pca_norm_rotate_args`` of include/pca_features.h."""
+    _fields_ = (
+        [(n, _vp) for n in ("q", "k")]
+        + [(n, _i64) for n in ("q_row", "q_head", "k_row", "k_head")]
+        + [(n, _vp) for n in ("weight_q", "weight_k", "pos", "freq")]
+        + [("rows", _i64)]
+        + [(n, ctypes.c_int32) for n in ("hq", "hk", "d", "axes", "rotated",
+                                         "dtype", "weight_dtype")]
+        + [("eps", ctypes.c_float)])
+
+
+# name -> (restype, argtypes); mirrors include/pca_features.h
+FEATURES_C_ABI = {
+    "pca_spans": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp]),
+    "pca_attention_workspace_bytes": (
+        ctypes.c_size_t, [_i64, _i64, ctypes.c_int32, ctypes.c_int32,
+                          ctypes.c_int32, ctypes.c_int]),
+    "pca_attention_forward": (
+        ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp, _vp, _vp,
+                       ctypes.c_size_t, _vp]),
+    "pca_attention_backward": (
+        ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp, _vp, _vp, _i64, _i64,
+                       _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    "pca_norm_rotate_forward": (
+        ctypes.c_int, [ctypes.POINTER(NormRotateArgs), _vp, _vp, _vp]),
+    "pca_norm_rotate_workspace_bytes": (ctypes.c_size_t,
+                                        [_i64, ctypes.c_int32]),
+    "pca_norm_rotate_backward": (
+        ctypes.c_int, [ctypes.POINTER(NormRotateArgs), _vp, _i64, _i64, _vp,
+                       _i64, _i64, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                       _vp]),
+    "pca_lookup": (
+        ctypes.c_int, [_vp, _vp, ctypes.c_int32, _i64, _i64, _i64,
+                       ctypes.c_float, ctypes.c_int32, _vp, _vp]),
+    "pca_lookup_grad_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64]),
+    "pca_lookup_grad": (
+        ctypes.c_int, [_vp, _vp, ctypes.c_int32, _i64, _i64, _i64,
+                       ctypes.c_float, ctypes.c_int32, _vp, _vp,
+                       ctypes.c_size_t, _vp]),
+}
+
+
 def load_capi():
     if not os.path.exists(CAPI_PATH):
         raise ImportError("%s is missing; %s" % (CAPI_PATH, _BUILD_HINT))
     lib = ctypes.CDLL(CAPI_PATH, mode=ctypes.RTLD_GLOBAL)
-    for name, (restype, argtypes) in C_ABI.items():
+    for name, (restype, argtypes) in {**C_ABI, **FEATURES_C_ABI}.items():
         fn = getattr(lib, name)
         fn.restype = restype
         fn.argtypes = argtypes

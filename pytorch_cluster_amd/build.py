@@ -5,7 +5,8 @@
 (run as a script: importing the package needs the libraries built here)
 
 Outputs (next to this file, git-ignored):
-  libpca_neighbors.so   HIP kernels + the C ABI of include/pca_neighbors.h
+  libpca_neighbors.so   HIP kernels + the C ABI of include/pca_neighbors.h and
+                        include/pca_features.h
   _torch_ops.so         TorchScript operator binding (links the above)
   libpca_probe.so       csrc/probes/: measurement and checking aids
                         (`bench.py --probe`, the bf16 rounding check of
@@ -106,7 +107,8 @@ def build_torch_ops():
         "-D_GLIBCXX_USE_CXX11_ABI=%d" % abi, "-Wno-deprecated-declarations",
         "-I", "/opt/rocm/include",
     ] + includes + [
-        os.path.join(CSRC, "torch_ops.cpp"), "-o", TORCH_OPS_LIB,
+        os.path.join(CSRC, "torch_ops.cpp"),
+        os.path.join(CSRC, "feature_ops.cpp"), "-o", TORCH_OPS_LIB,
         "-L", HERE, "-lpca_neighbors",
         "-L", torch_lib, "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10",
         "-lc10_hip", "-lamdhip64",

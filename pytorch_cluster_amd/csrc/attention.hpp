@@ -1,0 +1,81 @@
+// What the attention kernels (attention_impl.hpp), their dispatch (attention.hip) and
+// the C ABI (features_capi.hip) share.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace pca {
+
+// One side of an attention: [rows, heads, d] elements, the last dimension dense.
+struct HeadRows {
+  const void *data = nullptr;
+  int64_t row = 0, head = 0; // strides in elements
+  bool vec = false; // every row starts on 16 bytes and is a multiple of 16 long
+};
+
+struct AttentionCall {
+  HeadRows q, k, v;
+  const int2 *spans_q = nullptr; // rows of k that belong to a row of q: [begin,
+                                 // end) ([nq]; NULL: all of them)
+  const int2 *spans_k = nullptr; // the same for a row of k ([nk])
+  const float *pos_q = nullptr, *pos_k = nullptr; // [nq, axes], [nk, axes]
+  const float *slope = nullptr;                   // [hq]; NULL: no bias
+  int axes = 0;
+  int nq = 0, nk = 0, hq = 0, hk = 0, d = 0;
+  float scale = 1.f, cap = 0.f;
+
+  void *out = nullptr; // [nq, hq, d], dense
+  float *lse = nullptr; // [hq, nq]: log2 of the sum of exp2 of the scores (in
+                        // units of log 2); +inf for a row without keys
+
+  // backward
+  const void *out_in = nullptr;
+  HeadRows dout;
+  void *dq = nullptr, *dk = nullptr, *dv = nullptr; // dense
+  float *delta = nullptr;                           // [hq, nq]
+
+  // the looped side cut into pieces that meet in a kernel of their own
+  int splits = 1;
+  float *part = nullptr;    // forward, dq: [splits, nq, hq, d]; dk, dv:
+                            // [splits, 2, nk, hk, d]
+  float *part_ml = nullptr; // forward: [splits, nq, hq, 2]
+};
+
+// Which of the kernels of a pass runs, and in how many pieces.
+struct AttentionPlan {
+  bool wide = true;
+  int splits = 1;
+};
+
+// One per element type (0 fp32, 2 fp16, 3 bf16: pca_dtype) and width of a head (32,
+// 64, 128): attention_<type>_d<width>.hip.  `pass`: 0 forward, 1 dq, 2 dk and dv.
+typedef hipError_t (*AttentionLauncher)(const AttentionCall &, int pass,
+                                        bool wide, hipStream_t);
+#define PCA_ATTENTION_DECLARE(type)                                            \
+  hipError_t attention_##type##_d32(const AttentionCall &, int, bool,          \
+                                    hipStream_t);                              \
+  hipError_t attention_##type##_d64(const AttentionCall &, int, bool,          \
+                                    hipStream_t);                              \
+  hipError_t attention_##type##_d128(const AttentionCall &, int, bool,         \
+                                     hipStream_t)
+PCA_ATTENTION_DECLARE(f32);
+PCA_ATTENTION_DECLARE(f16);
+PCA_ATTENTION_DECLARE(bf16);
+#undef PCA_ATTENTION_DECLARE
+
+constexpr int kAttentionMaxD = 128;
+
+AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk);
+size_t attention_workspace_bytes(int pass, int64_t nq, int64_t nk, int hq,
+                                 int hk, int d);
+// workspace: of attention_workspace_bytes(0, ...) / (1, ...)
+hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
+                             hipStream_t stream);
+hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
+                              hipStream_t stream);
+hipError_t attention_spans(const int64_t *ids_a, int na, const int64_t *ids_b,
+                           int nb, int2 *spans, hipStream_t stream);
+
+} // namespace pca

@@ -1,0 +1,9 @@
+// Attention kernels: f32, heads of up to 32.
+#include "attention_impl.hpp"
+
+namespace pca {
+hipError_t attention_f32_d32(const AttentionCall &c, int pass, bool wide,
+                  hipStream_t stream) {
+  return attn::launch<float, 32>(c, pass, wide, stream);
+}
+} // namespace pca

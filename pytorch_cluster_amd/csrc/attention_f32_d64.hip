@@ -1,0 +1,9 @@
+// Attention kernels: f32, heads of up to 64.
+#include "attention_impl.hpp"
+
+namespace pca {
+hipError_t attention_f32_d64(const AttentionCall &c, int pass, bool wide,
+                  hipStream_t stream) {
+  return attn::launch<float, 64>(c, pass, wide, stream);
+}
+} // namespace pca

@@ -1,0 +1,1298 @@
+// Attention inside the examples of a batch: forward and backward kernels.
+//
+//   t_ij = scale q_i . k_j          u = cap tanh(t / cap)   (cap > 0; else u = t)
+//   s_ij = u - slope_h |p_i - p_j|  over the rows j of row i's example
+//   o_i  = sum_j exp(s_ij) v_j / sum_j exp(s_ij)
+//
+// and backwards, with P = exp(s - log sum exp s), delta_i = do_i . o_i:
+//
+//   dS = P (do_i . v_j - delta_i)   dT = dS (1 - (u / cap)^2)
+//   dq = scale sum_j dT k_j   dk = scale sum_i dT q_i   dv = sum_i P do_i
+//
+// Everything a kernel sums over lies along the matrix instruction's contraction and
+// everything it owns along its columns: scores are formed transposed, S^T = K Q^T, so
+// that a lane holds scores of ONE owned row (its column, lane % 16) and four
+// neighbouring looped rows per 16 x 16 block.  The row's maximum and sum are then
+// registers plus two exchanges between lanes, and the block's registers are already the
+// right operand of the next product (O^T += V^T P^T): the order of the contraction is
+// free as long as both operands use the same, so slot 8 g + j of a 32-wide step stands
+// for row 16 (j / 4) + 4 g + j % 4 of the step, which is what the lane holds.  The left
+// operand V^T comes transposed out of LDS (ds_read_tr16_b64) from rows stored as they
+// are in memory.  In fp32 the matrix instruction takes one element per lane and the
+// same layouts hold with steps of 16.
+//
+// Owned rows of the forward and of dq are (query, head of the group) pairs, so that the
+// heads that share a key head share its tiles as well; the kernel of dk and dv owns
+// keys and loops over those pairs.  No atomics: the same call gives the same bits.
+//
+// A tile of owned rows may touch several examples.  Its spans (begin and end of each
+// row's partner rows) are collected first; every span is walked in tiles of its own
+// that hold nothing of another example (rows beyond it are zeros), and where a wave's
+// columns belong to several examples the products are kept only in the columns that
+// the span belongs to: values of other examples, infinities and NaN among them, reach
+// nothing.
+#pragma once
+
+#include "attention.hpp"
+#include "device_utils.hpp"
+
+#include <type_traits>
+
+namespace pca {
+namespace attn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kThreads = 256, kWaves = 4;
+
+template <typename T> __device__ __forceinline__ float to_float(T v) {
+  return (float)v;
+}
+
+// acc += a b: both operands 16 bytes of a lane, element 0 of the contraction first.
+template <typename T>
+__device__ __forceinline__ void mma(f32x4 &acc, u32x4 a, u32x4 b) {
+  if constexpr (std::is_same<T, float>::value) {
+    const f32x4 fa = __builtin_bit_cast(f32x4, a);
+    const f32x4 fb = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      acc = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[c], fb[c], acc, 0, 0, 0);
+  } else if constexpr (std::is_same<T, _Float16>::value) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        __builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), acc, 0, 0,
+        0);
+  } else {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), acc, 0,
+        0, 0);
+  }
+}
+
+// Sizes that follow from the element type and the (padded) width of a head.
+template <typename T, int DP> struct Shape {
+  static constexpr int SZ = sizeof(T);
+  static constexpr int PER = 16 / SZ;          // elements of 16 bytes
+  static constexpr int CH = DP / PER;          // 16-byte pieces of a row
+  static constexpr int KS = CH / 4;            // steps of a product over d
+  static constexpr int DB = DP / 16;           // 16-wide blocks over d
+  static constexpr int PITCH = DP * SZ + 16;   // bytes of a row in LDS: 16 rows
+                                               // start on 16 different banks
+  static constexpr int KF = SZ == 2 ? 32 : 16; // rows of a step over rows
+  static constexpr int FB = KF / 16;           // ... in blocks
+};
+
+// 16 bytes of row `row` at piece `piece`; zeros beyond d.
+template <typename T, int DP>
+__device__ __forceinline__ u32x4 load_piece(const HeadRows &x, int64_t row,
+                                            int head, int piece, int d) {
+  constexpr int PER = Shape<T, DP>::PER;
+  const T *p = static_cast<const T *>(x.data) + row * x.row +
+               (int64_t)head * x.head + piece * PER;
+  u32x4 r = {0, 0, 0, 0};
+  if (x.vec) {
+    if (piece * PER < d)
+      r = *reinterpret_cast<const u32x4 *>(p);
+  } else {
+    T e[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      e[i] = piece * PER + i < d ? p[i] : (T)0.f;
+    __builtin_memcpy(&r, e, 16);
+  }
+  return r;
+}
+
+// ROWS rows of [begin, end) on their way from memory to LDS.  A row stands for
+// (row / group, head0 + row % group).
+template <typename T, int DP, int ROWS> struct Stage {
+  using S = Shape<T, DP>;
+  static constexpr int N = ROWS * S::CH / kThreads;
+  static_assert(ROWS * S::CH % kThreads == 0, "tile does not fill the threads");
+  u32x4 v[N];
+
+  __device__ __forceinline__ void load(const HeadRows &x, int begin, int end,
+                                       int group, int head0, int d) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * kThreads;
+      const int row = begin + c / S::CH;
+      v[i] = u32x4{0, 0, 0, 0};
+      if (row < end) {
+        const int r = group == 1 ? row : row / group;
+        v[i] = load_piece<T, DP>(x, r, head0 + row - r * group, c % S::CH, d);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char *tile) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int c = threadIdx.x + i * kThreads;
+      *reinterpret_cast<u32x4 *>(tile + (c / S::CH) * S::PITCH +
+                                 (c % S::CH) * 16) = v[i];
+    }
+  }
+};
+
+// Left operand with the tile's rows as its rows: row block `block`, step `ks` of d.
+template <typename T, int DP>
+__device__ __forceinline__ u32x4 rows_operand(const char *tile, int block,
+                                              int ks) {
+  const int lane = threadIdx.x & 63;
+  return *reinterpret_cast<const u32x4 *>(
+      tile + (block * 16 + (lane & 15)) * Shape<T, DP>::PITCH + ks * 64 +
+      (lane >> 4) * 16);
+}
+
+// Left operand with d as its rows (16 from d0) and the tile's rows from `row0` as the
+// contraction, in the order described above.
+template <typename T, int DP>
+__device__ __forceinline__ u32x4 turned_operand(const char *tile, int row0,
+                                                int db) {
+  using S = Shape<T, DP>;
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  if constexpr (S::SZ == 4) {
+    u32x4 r;
+    const char *p = tile + (row0 + g * 4) * S::PITCH + (db * 16 + i) * 4;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      r[c] = *reinterpret_cast<const uint32_t *>(p + c * S::PITCH);
+    return r;
+  } else {
+    // lane i of a group of 16 names 4 elements of row i / 4 and gets column i of
+    // the 4 x 16 elements that the group names
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const char *p =
+        tile + (row0 + g * 4 + (i >> 2)) * S::PITCH + (db * 16 + (i & 3) * 4) * 2;
+    const s16x4 lo =
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s16x4 *)(p + 16 * S::PITCH));
+    const u32x2 a = __builtin_bit_cast(u32x2, lo);
+    const u32x2 b = __builtin_bit_cast(u32x2, hi);
+    return u32x4{a[0], a[1], b[0], b[1]};
+  }
+}
+
+// Right operand of a step over the looped rows from the blocks that a lane holds.
+// Rounded to the element type: the matrix cores take nothing wider with 16-bit rows.
+// Their sums stay in 32 bits.
+template <typename T>
+__device__ __forceinline__ u32x4 block_operand(const f32x4 *blocks) {
+  if constexpr (std::is_same<T, float>::value) {
+    return __builtin_bit_cast(u32x4, blocks[0]);
+  } else {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      e[i] = (T)blocks[i >> 2][i & 3];
+    u32x4 r;
+    __builtin_memcpy(&r, e, 16);
+    return r;
+  }
+}
+
+// Four neighbouring elements of an output row.
+template <typename T>
+__device__ __forceinline__ void store4(T *p, f32x4 v, int left, bool vec) {
+  T e[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    e[i] = (T)v[i];
+  if (vec && left >= 4) {
+    __builtin_memcpy(__builtin_assume_aligned(p, 4 * sizeof(T)), e, sizeof(e));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left)
+        p[i] = e[i];
+  }
+}
+
+__device__ __forceinline__ float across_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16));
+  return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+  v += __shfl_xor(v, 16);
+  return v + __shfl_xor(v, 32);
+}
+
+// tanh(x / 2 log2 e)... of a score: t = tanh of `x` times log 2 / 2, that is
+// (exp2(x) - 1) / (exp2(x) + 1).  Near 0 the difference would lose what fp32 rows
+// need, so there the series is used: x log 2 / 2 below 0.35 (error 2e-8 relative).
+template <typename T> __device__ __forceinline__ float tanh_of(float x) {
+  const float e = __builtin_amdgcn_exp2f(x);
+  const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+  if constexpr (std::is_same<T, float>::value) {
+    const float y = x * 0.34657359027997264f, z = y * y;
+    const float near =
+        y + y * z *
+                (-0.33333333333f +
+                 z * (0.13333333333f +
+                      z * (-0.05396825397f +
+                           z * (0.02186948854f + z * -0.00886323553f))));
+    return fabsf(y) < 0.35f ? near : far;
+  }
+  return far;
+}
+
+// Spans of the rows that a workgroup owns, in order, each cut into tiles.
+template <int ROWS> struct Spans {
+  int begin[ROWS], end[ROWS];
+  int first[ROWS + 1]; // tiles before a span
+  int count;
+};
+
+// Collects the spans of owned rows [row0, row0 + ROWS) (row / group is the row that has
+// a span), whole workgroup; `scale`: looped rows per entry of a span, `tile`: of a tile.
+template <int ROWS>
+__device__ __forceinline__ void
+collect_spans(Spans<ROWS> &s, const int2 *spans, int row0, int rows, int group,
+              int all, int scale, int tile) {
+  if (spans == nullptr) {
+    if (threadIdx.x == 0) {
+      s.begin[0] = 0;
+      s.end[0] = all * scale;
+      s.first[0] = 0;
+      s.first[1] = (all * scale + tile - 1) / tile;
+      s.count = 1;
+    }
+    __syncthreads();
+    return;
+  }
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    int count = 0;
+    int2 last = make_int2(-1, -1);
+#pragma unroll
+    for (int base = 0; base < ROWS; base += 64) {
+      const int row = row0 + base + lane;
+      const bool there = base + lane < ROWS && row < rows;
+      int2 v = make_int2(-1, -1);
+      if (there)
+        v = spans[row / group];
+      int2 before;
+      before.x = __shfl_up(v.x, 1);
+      before.y = __shfl_up(v.y, 1);
+      if (lane == 0)
+        before = last;
+      const bool head = there && v.x < v.y &&
+                        (v.x != before.x || v.y != before.y);
+      const unsigned long long heads = __ballot(head);
+      if (head) {
+        const int at = count + __popcll(heads & ((1ull << lane) - 1));
+        s.begin[at] = v.x * scale;
+        s.end[at] = v.y * scale;
+      }
+      count += __popcll(heads);
+      last.x = __shfl(v.x, 63);
+      last.y = __shfl(v.y, 63);
+    }
+    if (lane == 0) {
+      s.count = count;
+      s.first[0] = 0;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int sum = 0;
+    for (int i = 0; i < s.count; ++i) {
+      sum += (s.end[i] - s.begin[i] + tile - 1) / tile;
+      s.first[i + 1] = sum;
+    }
+  }
+  __syncthreads();
+}
+
+// The tiles of this workgroup's piece, in order.
+template <int ROWS> struct Walk {
+  const Spans<ROWS> &s;
+  int at, stop, span, tile;
+  __device__ __forceinline__ Walk(const Spans<ROWS> &spans, int piece,
+                                  int pieces, int tile_rows)
+      : s(spans), tile(tile_rows) {
+    const int total = s.count > 0 ? s.first[s.count] : 0;
+    at = (int)((int64_t)total * piece / pieces);
+    stop = (int)((int64_t)total * (piece + 1) / pieces);
+    span = 0;
+    settle();
+  }
+  __device__ __forceinline__ void settle() {
+    if (at < stop)
+      while (s.first[span + 1] <= at)
+        ++span;
+  }
+  __device__ __forceinline__ bool there() const { return at < stop; }
+  __device__ __forceinline__ int begin() const {
+    return s.begin[span] + (at - s.first[span]) * tile;
+  }
+  __device__ __forceinline__ int end() const { return s.end[span]; }
+  __device__ __forceinline__ void next() {
+    ++at;
+    settle();
+  }
+};
+
+// The work of workgroup `block`: which tile of owned rows, which key head, which piece
+// of the looped rows.  Workgroups of an XCD (every eighth) take neighbouring tiles of
+// the same key head: they read the same rows, through one L2.
+struct Place {
+  int tile, head, piece;
+  __device__ __forceinline__ Place(int tiles, int heads, int pieces) {
+    // (blocks of an XCD: a grid that is no multiple of 8 leaves the first ones one
+    // more)
+    const int grid = tiles * heads * pieces, x = blockIdx.x & 7;
+    const int b = x * (grid >> 3) + min(x, grid & 7) + (blockIdx.x >> 3);
+    piece = b % pieces;
+    tile = b / pieces % tiles;
+    head = b / pieces / tiles;
+  }
+};
+
+// Rows of looped tiles per wave and step: the tile's 16-byte pieces fill the threads.
+template <typename T, int WK> struct Looped {
+  static constexpr int wave = WK == 1 ? (sizeof(T) == 2 ? 64 : 32)
+                                      : (sizeof(T) == 2 ? 32 : 16);
+  static constexpr int tile = wave * WK;
+};
+
+// A lane's owned column.
+struct Column {
+  bool valid = false;
+  int row = 0, head = 0; // of the query or key tensor
+  int2 span = {0, 0};
+  float slope = 0.f; // times log2 e
+  float p[3] = {0.f, 0.f, 0.f};
+};
+
+__device__ __forceinline__ void load_position(float (&p)[3], const float *pos,
+                                              int64_t row, int axes) {
+#pragma unroll
+  for (int a = 0; a < 3; ++a)
+    p[a] = a < axes ? pos[row * axes + a] : 0.f;
+}
+
+__device__ __forceinline__ Column query_column(const AttentionCall &c, int row,
+                                               int group, int head0) {
+  Column r;
+  r.valid = row < c.nq * group;
+  if (r.valid) {
+    r.row = row / group;
+    r.head = head0 + row % group;
+    r.span = c.spans_q ? c.spans_q[r.row] : make_int2(0, c.nk);
+    if (c.slope) {
+      r.slope = c.slope[r.head] * kLog2e;
+      load_position(r.p, c.pos_q, r.row, c.axes);
+    }
+  }
+  return r;
+}
+
+// Scores of a block in units of log 2, from the products; `key`: positions of the four
+// looped rows, `slope` per row.  Leaves 1 - tanh^2 in `flat` if asked for.
+template <typename T, bool FLAT>
+__device__ __forceinline__ void
+scores(f32x4 &s, const AttentionCall &c, const float (&p)[3],
+       const f32x4 (&other)[3], f32x4 slope, f32x4 *flat) {
+  if (c.cap > 0.f) {
+    const float in = c.scale / c.cap * (2.f * kLog2e), out = c.cap * kLog2e;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float t = tanh_of<T>(s[r] * in);
+      s[r] = t * out;
+      if (FLAT)
+        (*flat)[r] = 1.f - t * t;
+    }
+  } else {
+    s *= c.scale * kLog2e;
+  }
+  if (c.slope) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x = p[0] - other[0][r];
+      float d2 = x * x;
+      if (c.axes > 1) {
+        const float y = p[1] - other[1][r], z = p[2] - other[2][r];
+        d2 = fmaf(z, z, fmaf(y, y, d2));
+        d2 = __builtin_amdgcn_sqrtf(d2);
+      } else {
+        d2 = fabsf(x);
+      }
+      s[r] = fmaf(-slope[r], d2, s[r]);
+    }
+  }
+}
+
+// ---- forward ------------------------------------------------------------------
+
+// Rows of a wave's columns: RB blocks of 16.  WK waves share the same columns and
+// divide every tile among them (few rows); the others own columns of their own.
+template <typename T, int DP, int RB, int WK>
+__global__ __launch_bounds__(kThreads) void
+attention_forward_kernel(AttentionCall c) {
+  using S = Shape<T, DP>;
+  constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
+  constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
+  constexpr int KB = KW / 16;
+  constexpr int TILE = KT * S::PITCH;
+  __shared__ __attribute__((aligned(16))) char lds_tiles[2 * TILE];
+  char *const lds_k = lds_tiles, *const lds_v = lds_tiles + TILE;
+  __shared__ __attribute__((aligned(16))) float lds_pos[3][KT];
+  __shared__ float lds_ml[kWaves][16][2];
+  __shared__ Spans<ROWS> spans;
+
+  const int group = c.hq / c.hk, rows = c.nq * group;
+  const Place place((rows + ROWS - 1) / ROWS, c.hk, c.splits);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = lane & 15, g = lane >> 4;
+  const int wq = wave / WK, part = wave % WK * KW;
+  const int row0 = place.tile * ROWS;
+  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
+
+  Column col[RB];
+  u32x4 q[RB][S::KS];
+  f32x4 acc[S::DB][RB];
+  float m[RB], l[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    col[rb] = query_column(c, row0 + (wq * RB + rb) * 16 + i, group,
+                           place.head * group);
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks) {
+      q[rb][ks] = u32x4{0, 0, 0, 0};
+      if (col[rb].valid)
+        q[rb][ks] = load_piece<T, DP>(c.q, col[rb].row, col[rb].head,
+                                      ks * 4 + g, c.d);
+    }
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db)
+      acc[db][rb] = f32x4{0, 0, 0, 0};
+    m[rb] = -__builtin_inff();
+    l[rb] = 0.f;
+  }
+
+  Stage<T, DP, KT> stage_k, stage_v;
+  float stage_pos[3];
+  auto fetch = [&](int begin, int end) {
+    stage_k.load(c.k, begin, end, 1, place.head, c.d);
+    stage_v.load(c.v, begin, end, 1, place.head, c.d);
+    if (c.slope && threadIdx.x < KT) {
+      stage_pos[0] = stage_pos[1] = stage_pos[2] = 0.f;
+      const int row = begin + threadIdx.x;
+      if (row < end)
+        load_position(stage_pos, c.pos_k, row, c.axes);
+    }
+  };
+
+  Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  if (walk.there())
+    fetch(walk.begin(), walk.end());
+  while (walk.there()) {
+    const int begin = walk.begin(), end = walk.end();
+    const int2 span = make_int2(spans.begin[walk.span], end);
+    __syncthreads();
+    stage_k.store(lds_k);
+    stage_v.store(lds_v);
+    if (c.slope && threadIdx.x < KT) {
+#pragma unroll
+      for (int a = 0; a < 3; ++a)
+        lds_pos[a][threadIdx.x] = stage_pos[a];
+    }
+    __syncthreads();
+    walk.next();
+    if (walk.there())
+      fetch(walk.begin(), walk.end());
+
+    bool in[RB];
+    bool any = false, all = true;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      in[rb] = col[rb].span.x == span.x && col[rb].span.y == span.y;
+      any |= in[rb] && col[rb].valid;
+      all &= in[rb] || !col[rb].valid;
+    }
+    if (__ballot(any) == 0 || begin + part >= end)
+      continue;
+    const bool mixed = __ballot(!all) != 0;
+    const bool cut = begin + part + KW > end;
+
+    f32x4 s[RB][KB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+        s[rb][kb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int ks = 0; ks < S::KS; ++ks) {
+        const u32x4 a =
+            rows_operand<T, DP>(lds_k + part * S::PITCH, kb, ks);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          mma<T>(s[rb][kb], a, q[rb][ks]);
+      }
+
+    float top[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+      top[rb] = -__builtin_inff();
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      f32x4 pos[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+      const int at = part + kb * 16 + g * 4;
+      if (c.slope) {
+#pragma unroll
+        for (int a = 0; a < 3; ++a)
+          pos[a] = *reinterpret_cast<const f32x4 *>(&lds_pos[a][at]);
+      }
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const float sl = col[rb].slope;
+        scores<T, false>(s[rb][kb], c, col[rb].p, pos, f32x4{sl, sl, sl, sl},
+                         nullptr);
+        if (cut || mixed) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!in[rb] || begin + at + r >= end)
+              s[rb][kb][r] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          top[rb] = fmaxf(top[rb], s[rb][kb][r]);
+      }
+    }
+
+    // The maximum that is subtracted moves only when it would grow by more than 8
+    // (256-fold sums, far from any limit): most tiles leave the sums as they are.
+    bool grow = false;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      top[rb] = across_groups_max(top[rb]);
+      grow |= top[rb] > m[rb] + 8.f;
+    }
+    if (__ballot(grow) != 0) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        const float now = fmaxf(m[rb], top[rb]);
+        const float keep = now == -__builtin_inff()
+                               ? 1.f
+                               : __builtin_amdgcn_exp2f(m[rb] - now);
+        m[rb] = now;
+        l[rb] *= keep;
+#pragma unroll
+        for (int db = 0; db < S::DB; ++db)
+          acc[db][rb] *= keep;
+      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      const float base = m[rb] == -__builtin_inff() ? 0.f : m[rb];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = __builtin_amdgcn_exp2f(s[rb][kb][r] - base);
+          s[rb][kb][r] = e;
+          l[rb] += e;
+        }
+    }
+
+#pragma unroll
+    for (int f = 0; f < KB / S::FB; ++f) {
+      u32x4 p[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        p[rb] = block_operand<T>(&s[rb][f * S::FB]);
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        const u32x4 a = turned_operand<T, DP>(lds_v, part + f * S::KF, db);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          if (mixed) {
+            f32x4 t = acc[db][rb];
+            mma<T>(t, a, p[rb]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              acc[db][rb][r] = in[rb] ? t[r] : acc[db][rb][r];
+          } else {
+            mma<T>(acc[db][rb], a, p[rb]);
+          }
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+    l[rb] = across_groups_sum(l[rb]);
+
+  if constexpr (WK > 1) {
+    // the waves' shares of the same 16 columns: one maximum, then sums in the order
+    // of the waves
+    static_assert(RB == 1 && WQ == 1, "one block of columns");
+    static_assert(kWaves * 16 * (DP + 4) * 4 <= 2 * TILE, "sums do not fit");
+    auto lds_acc = reinterpret_cast<float(*)[16][DP + 4]>(lds_tiles);
+    if (g == 0) {
+      lds_ml[wave][i][0] = m[0];
+      lds_ml[wave][i][1] = l[0];
+    }
+    __syncthreads();
+    float top = -__builtin_inff(), sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w)
+      top = fmaxf(top, lds_ml[w][i][0]);
+#pragma unroll
+    for (int w = 0; w < WK; ++w)
+      if (lds_ml[w][i][0] != -__builtin_inff())
+        sum += lds_ml[w][i][1] * __builtin_amdgcn_exp2f(lds_ml[w][i][0] - top);
+    const float keep = m[0] == -__builtin_inff()
+                           ? 1.f
+                           : __builtin_amdgcn_exp2f(m[0] - top);
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db)
+      *reinterpret_cast<f32x4 *>(&lds_acc[wave][i][db * 16 + g * 4]) =
+          acc[db][0] * keep;
+    __syncthreads();
+    m[0] = top;
+    l[0] = sum;
+    // wave w finishes blocks w, w + 4, ... of d
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db) {
+      f32x4 t = {0, 0, 0, 0};
+      if (db % kWaves == wave) {
+#pragma unroll
+        for (int w = 0; w < WK; ++w)
+          t += *reinterpret_cast<const f32x4 *>(&lds_acc[w][i][db * 16 + g * 4]);
+      }
+      acc[db][0] = t;
+    }
+  }
+
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    if (!col[rb].valid)
+      continue;
+    const int64_t at = (int64_t)col[rb].row * c.hq + col[rb].head;
+    const bool vec = c.d % 4 == 0;
+    const bool first = g == 0 && (WK == 1 || wave == 0);
+    if (c.splits > 1) {
+      const int64_t o = (int64_t)place.piece * c.nq * c.hq + at;
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        if (WK > 1 && db % kWaves != wave)
+          continue;
+        const int e = db * 16 + g * 4;
+        store4<float>(c.part + o * c.d + e, acc[db][rb], c.d - e, vec);
+      }
+      if (first) {
+        c.part_ml[o * 2] = m[rb];
+        c.part_ml[o * 2 + 1] = l[rb];
+      }
+    } else {
+      const float inv = l[rb] == 0.f ? 0.f : 1.f / l[rb];
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        if (WK > 1 && db % kWaves != wave)
+          continue;
+        const int e = db * 16 + g * 4;
+        store4<T>(static_cast<T *>(c.out) + at * c.d + e, acc[db][rb] * inv,
+                  c.d - e, vec);
+      }
+      if (first && c.lse)
+        c.lse[(int64_t)col[rb].head * c.nq + col[rb].row] =
+            l[rb] == 0.f ? __builtin_inff()
+                         : m[rb] + __builtin_amdgcn_logf(l[rb]);
+    }
+  }
+}
+
+// ---- backward -----------------------------------------------------------------
+
+// Factors that keep dS inside fp16's range, one per column: a power of two that grows
+// or shrinks with the largest value met (bf16 and fp32 have the range of the sums and
+// need none).  Sums are kept times the factor.
+template <typename T> struct Range {
+  static constexpr bool on = std::is_same<T, _Float16>::value;
+  float factor = on ? 0x1p96f : 1.f;
+
+  // Before a step with values up to `top` (of the lane): what the sums so far have to
+  // be multiplied by.
+  __device__ __forceinline__ bool moves(float top) const {
+    return on && top * factor > 0x1p15f;
+  }
+  __device__ __forceinline__ float move(float top) {
+    top = across_groups_max(top);
+    if (!(top * factor > 0x1p15f))
+      return 1.f;
+    // (a finite top: exponents of values stay between those of fp32)
+    const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+    const float next = __uint_as_float((uint32_t)(min(127 + 12 - e, 250)) << 23);
+    const float by = next / factor;
+    if (e == 128)
+      return 1.f; // an infinity or NaN stays what it is
+    factor = next;
+    return by;
+  }
+};
+
+// Probabilities go to fp16 products times 2^14 (at most 1, and as small as one in the
+// number of rows).
+template <typename T>
+constexpr float kWeightUp = std::is_same<T, _Float16>::value ? 0x1p14f : 1.f;
+
+// Sums of a wave's columns: blocks of d, blocks of columns.
+template <typename T, int DP, int RB> using Sums = f32x4[Shape<T, DP>::DB][RB];
+
+// WK waves' sums of the same 16 columns, in the order of the waves: afterwards wave w
+// holds blocks w, w + 4, ... of d.
+template <typename T, int DP, int RB, int WK>
+__device__ __forceinline__ void
+join_waves(Sums<T, DP, RB> &acc, float (*lds)[16][DP + 4]) {
+  if constexpr (WK > 1) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int i = lane & 15, g = lane >> 4;
+    __syncthreads();
+#pragma unroll
+    for (int db = 0; db < Shape<T, DP>::DB; ++db)
+      *reinterpret_cast<f32x4 *>(&lds[wave][i][db * 16 + g * 4]) = acc[db][0];
+    __syncthreads();
+#pragma unroll
+    for (int db = 0; db < Shape<T, DP>::DB; ++db) {
+      f32x4 t = {0, 0, 0, 0};
+      if (db % kWaves == wave) {
+#pragma unroll
+        for (int w = 0; w < WK; ++w)
+          t += *reinterpret_cast<const f32x4 *>(&lds[w][i][db * 16 + g * 4]);
+      }
+      acc[db][0] = t;
+    }
+  }
+}
+
+// A column's sums to memory: to the gradient, or to the piece's place.
+template <typename T, int DP, int RB, int WK>
+__device__ __forceinline__ void
+store_columns(const Sums<T, DP, RB> &acc, int rb, void *out, float *part,
+              int64_t at, int d, float factor) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4;
+  const bool vec = d % 4 == 0;
+#pragma unroll
+  for (int db = 0; db < Shape<T, DP>::DB; ++db) {
+    if (WK > 1 && db % kWaves != wave)
+      continue;
+    const int e = db * 16 + g * 4;
+    const f32x4 v = acc[db][rb] * factor;
+    if (part)
+      store4<float>(part + at * d + e, v, d - e, vec);
+    else
+      store4<T>(static_cast<T *>(out) + at * d + e, v, d - e, vec);
+  }
+}
+
+// dq of the rows that a workgroup owns, looping over keys; writes delta for the kernel
+// of dk and dv.
+template <typename T, int DP, int RB, int WK>
+__global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttentionCall c) {
+  using S = Shape<T, DP>;
+  constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
+  constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
+  constexpr int KB = KW / 16;
+  constexpr int TILE = KT * S::PITCH;
+  __shared__ __attribute__((aligned(16))) char lds_tiles[2 * TILE];
+  char *const lds_k = lds_tiles, *const lds_v = lds_tiles + TILE;
+  __shared__ __attribute__((aligned(16))) float lds_pos[3][KT];
+  __shared__ Spans<ROWS> spans;
+
+  const int group = c.hq / c.hk, rows = c.nq * group;
+  const Place place((rows + ROWS - 1) / ROWS, c.hk, c.splits);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = lane & 15, g = lane >> 4;
+  const int wq = wave / WK, part = wave % WK * KW;
+  const int row0 = place.tile * ROWS;
+  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
+
+  Column col[RB];
+  u32x4 q[RB][S::KS], dout[RB][S::KS];
+  f32x4 acc[S::DB][RB];
+  float lse[RB], delta[RB];
+  Range<T> range[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    col[rb] = query_column(c, row0 + (wq * RB + rb) * 16 + i, group,
+                           place.head * group);
+    HeadRows out;
+    out.data = c.out_in;
+    out.row = (int64_t)c.hq * c.d;
+    out.head = c.d;
+    out.vec = c.d * S::SZ % 16 == 0;
+    float sum = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks) {
+      q[rb][ks] = dout[rb][ks] = u32x4{0, 0, 0, 0};
+      if (col[rb].valid) {
+        const int piece = ks * 4 + g;
+        q[rb][ks] =
+            load_piece<T, DP>(c.q, col[rb].row, col[rb].head, piece, c.d);
+        dout[rb][ks] =
+            load_piece<T, DP>(c.dout, col[rb].row, col[rb].head, piece, c.d);
+        const u32x4 o =
+            load_piece<T, DP>(out, col[rb].row, col[rb].head, piece, c.d);
+        T a[S::PER], b[S::PER];
+        __builtin_memcpy(a, &o, 16);
+        __builtin_memcpy(b, &dout[rb][ks], 16);
+#pragma unroll
+        for (int e = 0; e < S::PER; ++e)
+          sum = fmaf(to_float(a[e]), to_float(b[e]), sum);
+      }
+    }
+    delta[rb] = across_groups_sum(sum);
+    lse[rb] = __builtin_inff();
+    if (col[rb].valid) {
+      const int64_t at = (int64_t)col[rb].head * c.nq + col[rb].row;
+      lse[rb] = c.lse[at];
+      if (place.piece == 0 && g == 0 && (WK == 1 || wave == 0))
+        c.delta[at] = delta[rb];
+    }
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db)
+      acc[db][rb] = f32x4{0, 0, 0, 0};
+  }
+
+  Stage<T, DP, KT> stage_k, stage_v;
+  float stage_pos[3];
+  auto fetch = [&](int begin, int end) {
+    stage_k.load(c.k, begin, end, 1, place.head, c.d);
+    stage_v.load(c.v, begin, end, 1, place.head, c.d);
+    if (c.slope && threadIdx.x < KT) {
+      stage_pos[0] = stage_pos[1] = stage_pos[2] = 0.f;
+      const int row = begin + threadIdx.x;
+      if (row < end)
+        load_position(stage_pos, c.pos_k, row, c.axes);
+    }
+  };
+
+  Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  if (walk.there())
+    fetch(walk.begin(), walk.end());
+  while (walk.there()) {
+    const int begin = walk.begin(), end = walk.end();
+    const int2 span = make_int2(spans.begin[walk.span], end);
+    __syncthreads();
+    stage_k.store(lds_k);
+    stage_v.store(lds_v);
+    if (c.slope && threadIdx.x < KT) {
+#pragma unroll
+      for (int a = 0; a < 3; ++a)
+        lds_pos[a][threadIdx.x] = stage_pos[a];
+    }
+    __syncthreads();
+    walk.next();
+    if (walk.there())
+      fetch(walk.begin(), walk.end());
+
+    bool in[RB];
+    bool any = false, all = true;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      in[rb] = col[rb].span.x == span.x && col[rb].span.y == span.y;
+      any |= in[rb] && col[rb].valid;
+      all &= in[rb] || !col[rb].valid;
+    }
+    if (__ballot(any) == 0 || begin + part >= end)
+      continue;
+    const bool mixed = __ballot(!all) != 0;
+    const bool cut = begin + part + KW > end;
+
+#pragma unroll
+    for (int f = 0; f < KB / S::FB; ++f) {
+      f32x4 ds[RB][S::FB];
+      float top[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        top[rb] = 0.f;
+#pragma unroll
+      for (int b = 0; b < S::FB; ++b) {
+        const int kb = f * S::FB + b;
+        f32x4 s[RB], dp[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          s[rb] = dp[rb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ++ks) {
+          const u32x4 a = rows_operand<T, DP>(lds_k + part * S::PITCH, kb, ks);
+          const u32x4 b2 = rows_operand<T, DP>(lds_v + part * S::PITCH, kb, ks);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            mma<T>(s[rb], a, q[rb][ks]);
+            mma<T>(dp[rb], b2, dout[rb][ks]);
+          }
+        }
+        f32x4 pos[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
+        const int at = part + kb * 16 + g * 4;
+        if (c.slope) {
+#pragma unroll
+          for (int a = 0; a < 3; ++a)
+            pos[a] = *reinterpret_cast<const f32x4 *>(&lds_pos[a][at]);
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          const float sl = col[rb].slope;
+          f32x4 flat;
+          scores<T, true>(s[rb], c, col[rb].p, pos, f32x4{sl, sl, sl, sl},
+                          &flat);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float v = __builtin_amdgcn_exp2f(s[rb][r] - lse[rb]) *
+                      (dp[rb][r] - delta[rb]);
+            if (c.cap > 0.f)
+              v *= flat[r];
+            if ((cut || mixed) && (!in[rb] || begin + at + r >= end))
+              v = 0.f;
+            ds[rb][b][r] = v;
+            top[rb] = fmaxf(top[rb], fabsf(v));
+          }
+        }
+      }
+      if constexpr (Range<T>::on) {
+        bool moves = false;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          moves |= range[rb].moves(top[rb]);
+        if (__ballot(moves) != 0) {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            const float by = range[rb].move(top[rb]);
+#pragma unroll
+            for (int db = 0; db < S::DB; ++db)
+              acc[db][rb] *= by;
+          }
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+            ds[rb][b] *= range[rb].factor;
+      }
+      u32x4 p[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        p[rb] = block_operand<T>(ds[rb]);
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        const u32x4 a = turned_operand<T, DP>(lds_k, part + f * S::KF, db);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          if (mixed) {
+            f32x4 t = acc[db][rb];
+            mma<T>(t, a, p[rb]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              acc[db][rb][r] = in[rb] ? t[r] : acc[db][rb][r];
+          } else {
+            mma<T>(acc[db][rb], a, p[rb]);
+          }
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db)
+      acc[db][rb] *= 1.f / range[rb].factor;
+  if constexpr (WK > 1) {
+    static_assert(kWaves * 16 * (DP + 4) * 4 <= 2 * TILE, "sums do not fit");
+    auto lds_acc = reinterpret_cast<float(*)[16][DP + 4]>(lds_tiles);
+    join_waves<T, DP, RB, WK>(acc, lds_acc);
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+    if (col[rb].valid) {
+      const int64_t at = (int64_t)col[rb].row * c.hq + col[rb].head;
+      float *piece =
+          c.splits > 1
+              ? c.part + (int64_t)place.piece * c.nq * c.hq * c.d
+              : nullptr;
+      store_columns<T, DP, RB, WK>(acc, rb, c.dq, piece, at, c.d, c.scale);
+    }
+}
+
+// dk and dv of the keys that a workgroup owns, looping over (query, head) rows.
+template <typename T, int DP, int RB, int WK>
+__global__ __launch_bounds__(kThreads) void
+attention_dkv_kernel(AttentionCall c) {
+  using S = Shape<T, DP>;
+  constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
+  constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
+  constexpr int KB = KW / 16;
+  constexpr int TILE = KT * S::PITCH;
+  __shared__ __attribute__((aligned(16))) char lds_tiles[2 * TILE];
+  char *const lds_q = lds_tiles, *const lds_do = lds_tiles + TILE;
+  // per looped row: position, slope (times log2 e), lse, delta
+  __shared__ __attribute__((aligned(16))) float lds_row[6][KT];
+  __shared__ Spans<ROWS> spans;
+
+  const int group = c.hq / c.hk;
+  const Place place((c.nk + ROWS - 1) / ROWS, c.hk, c.splits);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int i = lane & 15, g = lane >> 4;
+  const int wq = wave / WK, part = wave % WK * KW;
+  const int row0 = place.tile * ROWS, head0 = place.head * group;
+  collect_spans<ROWS>(spans, c.spans_k, row0, c.nk, 1, c.nq, group, KT);
+
+  Column col[RB];
+  u32x4 k[RB][S::KS], v[RB][S::KS];
+  f32x4 acc_k[S::DB][RB], acc_v[S::DB][RB];
+  Range<T> range[RB];
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb) {
+    const int row = row0 + (wq * RB + rb) * 16 + i;
+    col[rb].valid = row < c.nk;
+    if (col[rb].valid) {
+      col[rb].row = row;
+      col[rb].span = c.spans_k ? c.spans_k[row] : make_int2(0, c.nq);
+      col[rb].span.x *= group;
+      col[rb].span.y *= group;
+      if (c.slope)
+        load_position(col[rb].p, c.pos_k, row, c.axes);
+    }
+#pragma unroll
+    for (int ks = 0; ks < S::KS; ++ks) {
+      k[rb][ks] = v[rb][ks] = u32x4{0, 0, 0, 0};
+      if (col[rb].valid) {
+        k[rb][ks] = load_piece<T, DP>(c.k, row, place.head, ks * 4 + g, c.d);
+        v[rb][ks] = load_piece<T, DP>(c.v, row, place.head, ks * 4 + g, c.d);
+      }
+    }
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db)
+      acc_k[db][rb] = acc_v[db][rb] = f32x4{0, 0, 0, 0};
+  }
+
+  Stage<T, DP, KT> stage_q, stage_do;
+  float stage_row[6];
+  auto fetch = [&](int begin, int end) {
+    stage_q.load(c.q, begin, end, group, head0, c.d);
+    stage_do.load(c.dout, begin, end, group, head0, c.d);
+    if (threadIdx.x < KT) {
+#pragma unroll
+      for (int a = 0; a < 6; ++a)
+        stage_row[a] = 0.f;
+      const int row = begin + threadIdx.x;
+      if (row < end) {
+        const int query = row / group, head = head0 + row % group;
+        if (c.slope) {
+          float p[3];
+          load_position(p, c.pos_q, query, c.axes);
+#pragma unroll
+          for (int a = 0; a < 3; ++a)
+            stage_row[a] = p[a];
+          stage_row[3] = c.slope[head] * kLog2e;
+        }
+        stage_row[4] = c.lse[(int64_t)head * c.nq + query];
+        stage_row[5] = c.delta[(int64_t)head * c.nq + query];
+      }
+    }
+  };
+
+  Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  if (walk.there())
+    fetch(walk.begin(), walk.end());
+  while (walk.there()) {
+    const int begin = walk.begin(), end = walk.end();
+    const int2 span = make_int2(spans.begin[walk.span], end);
+    __syncthreads();
+    stage_q.store(lds_q);
+    stage_do.store(lds_do);
+    if (threadIdx.x < KT) {
+#pragma unroll
+      for (int a = 0; a < 6; ++a)
+        lds_row[a][threadIdx.x] = stage_row[a];
+    }
+    __syncthreads();
+    walk.next();
+    if (walk.there())
+      fetch(walk.begin(), walk.end());
+
+    bool in[RB];
+    bool any = false, all = true;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      in[rb] = col[rb].span.x == span.x && col[rb].span.y == span.y;
+      any |= in[rb] && col[rb].valid;
+      all &= in[rb] || !col[rb].valid;
+    }
+    if (__ballot(any) == 0 || begin + part >= end)
+      continue;
+    const bool mixed = __ballot(!all) != 0;
+    const bool cut = begin + part + KW > end;
+
+#pragma unroll
+    for (int f = 0; f < KB / S::FB; ++f) {
+      f32x4 ds[RB][S::FB], pr[RB][S::FB];
+      float top[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        top[rb] = 0.f;
+#pragma unroll
+      for (int b = 0; b < S::FB; ++b) {
+        const int kb = f * S::FB + b;
+        f32x4 s[RB], dp[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          s[rb] = dp[rb] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ++ks) {
+          const u32x4 a = rows_operand<T, DP>(lds_q + part * S::PITCH, kb, ks);
+          const u32x4 b2 =
+              rows_operand<T, DP>(lds_do + part * S::PITCH, kb, ks);
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            mma<T>(s[rb], a, k[rb][ks]);
+            mma<T>(dp[rb], b2, v[rb][ks]);
+          }
+        }
+        f32x4 row[6];
+        const int at = part + kb * 16 + g * 4;
+#pragma unroll
+        for (int a = 0; a < 6; ++a)
+          row[a] = *reinterpret_cast<const f32x4 *>(&lds_row[a][at]);
+        const f32x4 pos[3] = {row[0], row[1], row[2]};
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          f32x4 flat;
+          scores<T, true>(s[rb], c, col[rb].p, pos, row[3], &flat);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float w = __builtin_amdgcn_exp2f(s[rb][r] - row[4][r]);
+            float x = w * (dp[rb][r] - row[5][r]);
+            if (c.cap > 0.f)
+              x *= flat[r];
+            if ((cut || mixed) && (!in[rb] || begin + at + r >= end))
+              w = x = 0.f;
+            pr[rb][b][r] = w * kWeightUp<T>;
+            ds[rb][b][r] = x;
+            top[rb] = fmaxf(top[rb], fabsf(x));
+          }
+        }
+      }
+      if constexpr (Range<T>::on) {
+        bool moves = false;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          moves |= range[rb].moves(top[rb]);
+        if (__ballot(moves) != 0) {
+#pragma unroll
+          for (int rb = 0; rb < RB; ++rb) {
+            const float by = range[rb].move(top[rb]);
+#pragma unroll
+            for (int db = 0; db < S::DB; ++db)
+              acc_k[db][rb] *= by;
+          }
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+            ds[rb][b] *= range[rb].factor;
+      }
+      u32x4 p[RB], x[RB];
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        p[rb] = block_operand<T>(pr[rb]);
+        x[rb] = block_operand<T>(ds[rb]);
+      }
+#pragma unroll
+      for (int db = 0; db < S::DB; ++db) {
+        const u32x4 a = turned_operand<T, DP>(lds_do, part + f * S::KF, db);
+        const u32x4 b = turned_operand<T, DP>(lds_q, part + f * S::KF, db);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          if (mixed) {
+            f32x4 t = acc_v[db][rb], u = acc_k[db][rb];
+            mma<T>(t, a, p[rb]);
+            mma<T>(u, b, x[rb]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              acc_v[db][rb][r] = in[rb] ? t[r] : acc_v[db][rb][r];
+              acc_k[db][rb][r] = in[rb] ? u[r] : acc_k[db][rb][r];
+            }
+          } else {
+            mma<T>(acc_v[db][rb], a, p[rb]);
+            mma<T>(acc_k[db][rb], b, x[rb]);
+          }
+        }
+      }
+    }
+  }
+
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db)
+      acc_k[db][rb] *= 1.f / range[rb].factor;
+  if constexpr (WK > 1) {
+    static_assert(kWaves * 16 * (DP + 4) * 4 <= 2 * TILE, "sums do not fit");
+    auto lds_acc = reinterpret_cast<float(*)[16][DP + 4]>(lds_tiles);
+    join_waves<T, DP, RB, WK>(acc_k, lds_acc);
+    join_waves<T, DP, RB, WK>(acc_v, lds_acc);
+  }
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+    if (col[rb].valid) {
+      const int64_t at = (int64_t)col[rb].row * c.hk + place.head;
+      const int64_t one = (int64_t)c.nk * c.hk * c.d;
+      float *piece = c.splits > 1 ? c.part + place.piece * 2 * one : nullptr;
+      store_columns<T, DP, RB, WK>(acc_k, rb, c.dk, piece, at, c.d, c.scale);
+      store_columns<T, DP, RB, WK>(acc_v, rb, c.dv, piece ? piece + one : nullptr,
+                                   at, c.d, 1.f / kWeightUp<T>);
+    }
+}
+
+// ---- launch -------------------------------------------------------------------
+
+// Owned rows of a workgroup.
+constexpr int kWideRows = 128, kFewRows = 16;
+
+template <typename T, int DP>
+hipError_t launch(const AttentionCall &c, int pass, bool wide,
+                  hipStream_t stream) {
+  const int64_t owned =
+      pass == 2 ? c.nk : (int64_t)c.nq * (c.hq / c.hk);
+  const int rows = wide ? kWideRows : kFewRows;
+  const int64_t grid = (owned + rows - 1) / rows * c.hk * c.splits;
+  if (grid <= 0)
+    return hipSuccess;
+  if (grid > INT32_MAX)
+    return hipErrorInvalidValue;
+  const dim3 g((unsigned)grid), b(kThreads);
+  if (pass == 0) {
+    if (wide)
+      attention_forward_kernel<T, DP, 2, 1><<<g, b, 0, stream>>>(c);
+    else
+      attention_forward_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
+  } else if (pass == 1) {
+    if (wide)
+      attention_dq_kernel<T, DP, 2, 1><<<g, b, 0, stream>>>(c);
+    else
+      attention_dq_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
+  } else {
+    if (wide)
+      attention_dkv_kernel<T, DP, 2, 1><<<g, b, 0, stream>>>(c);
+    else
+      attention_dkv_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
+  }
+  return hipGetLastError();
+}
+
+} // namespace attn
+} // namespace pca

@@ -19,10 +19,15 @@ namespace {
 
 thread_local char g_last_error[256] = "";
 
+int vfail(int status, const char *fmt, va_list ap) {
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  return status;
+}
+
 int fail(int status, const char *fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
-  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  vfail(status, fmt, ap);
   va_end(ap);
   return status;
 }
@@ -345,6 +350,18 @@ int fixed_scratch_of_current_device(void **out) {
 }
 
 } // namespace
+
+namespace pca {
+
+int fail(int status, const char *fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vfail(status, fmt, ap);
+  va_end(ap);
+  return status;
+}
+
+} // namespace pca
 
 extern "C" {
 

@@ -1,0 +1,608 @@
+// Rows of a table by index, out_e = scale table[index_e], and the gradient of the
+// table:
+//
+//   dtable_n = scale sum over e with index_e = n of dout_e
+//
+// An index outside the table names no row: its output row is zeros and it adds to no
+// gradient (places that a search left empty hold -1).
+//
+// The gradient is summed in 32 bits without atomics: the entries are sorted by index,
+// stable and by digits of up to 8 bits (entries of no row come last), and the sorted
+// list is cut into chunks of equal length whatever the rows are -- one row may have most
+// entries.  A group of lanes adds up a chunk, run after run; a run that lies in one
+// chunk goes straight to the gradient, the others leave their first and last sums in
+// the workspace, and the chunk where a run starts adds up its parts.  The same call
+// gives the same bits.
+#include "rows_ops.hpp"
+
+#include "attention_impl.hpp"
+
+#include <algorithm>
+
+namespace pca {
+
+namespace {
+
+constexpr int kSortThreads = 512, kPer = 8;
+constexpr int kTile = kSortThreads * kPer; // entries of a sorting workgroup
+constexpr int kBits = 8, kDigits = 1 << kBits;
+
+size_t lk_align(size_t v) { return (v + 255) & ~(size_t)255; }
+
+__device__ __forceinline__ int64_t index_at(const LookupCall &c, int64_t e) {
+  return c.wide_index ? static_cast<const int64_t *>(c.index)[e]
+                      : (int64_t) static_cast<const int32_t *>(c.index)[e];
+}
+// Sorting key of an entry: its row, `table` for none.
+__device__ __forceinline__ uint32_t key_at(const LookupCall &c, int64_t e) {
+  const int64_t i = index_at(c, e);
+  return (uint32_t)(i >= 0 && i < c.table ? i : c.table);
+}
+
+// ---- forward ------------------------------------------------------------------
+
+// A thread per 16 bytes of an output row.
+template <typename T>
+__global__ __launch_bounds__(256) void
+lookup_kernel(LookupCall c, int64_t pieces, int64_t total) {
+  constexpr int PER = 16 / (int)sizeof(T);
+  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total;
+       at += (int64_t)gridDim.x * 256) {
+    const int64_t e = at / pieces;
+    const int64_t e0 = (at - e * pieces) * PER;
+    const int64_t row = index_at(c, e);
+    T v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      v[i] = (T)0.f;
+    const bool there = row >= 0 && row < c.table;
+    const T *from = static_cast<const T *>(c.rows) + row * c.width + e0;
+    T *to = static_cast<T *>(c.out) + e * c.width + e0;
+    if (c.width % PER == 0) {
+      if (there) {
+        __builtin_memcpy(v, __builtin_assume_aligned(from, 16), 16);
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          v[i] = (T)((float)v[i] * c.scale);
+      }
+      __builtin_memcpy(__builtin_assume_aligned(to, 16), v, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (e0 + i < c.width)
+          to[i] = there ? (T)((float)from[i] * c.scale) : (T)0.f;
+    }
+  }
+}
+
+// ---- the entries in the order of their rows -------------------------------------
+
+struct Sorted {
+  uint64_t *a, *b;    // [entries] (key, entry), by turns
+  uint32_t *digits;   // [kDigits][tiles], then [kDigits] totals
+  uint32_t *keys, *perm; // [entries]: the result
+  int tiles;
+};
+
+struct Pass {
+  int number, shift, bits;
+  bool last;
+};
+
+__device__ __forceinline__ uint64_t pair_at(const LookupCall &c,
+                                            const Sorted &s, const Pass &p,
+                                            int e) {
+  if (p.number == 0)
+    return (uint64_t)key_at(c, e) << 32 | (uint32_t)e;
+  return (p.number & 1 ? s.a : s.b)[e];
+}
+
+// Entries of a tile by digit; in the first pass the whole grid also clears the
+// gradient (rows without entries keep the zeros).
+__global__ __launch_bounds__(kSortThreads) void
+lookup_count_kernel(LookupCall c, Sorted s, Pass p, int64_t clear) {
+  __shared__ uint32_t count[kDigits];
+  const int tid = threadIdx.x;
+  for (int64_t i = (int64_t)blockIdx.x * kSortThreads + tid; i < clear;
+       i += (int64_t)gridDim.x * kSortThreads)
+    static_cast<uint16_t *>(c.out)[i] = 0;
+  const int tile = blockIdx.x;
+  if (tile >= s.tiles)
+    return;
+  if (tid < kDigits)
+    count[tid] = 0u;
+  __syncthreads();
+  const uint32_t mask = (1u << p.bits) - 1;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t e = (int64_t)tile * kTile + i * kSortThreads + tid;
+    if (e < c.entries)
+      atomicAdd(&count[(uint32_t)(pair_at(c, s, p, (int)e) >> 32) >> p.shift &
+                       mask],
+                1u);
+  }
+  __syncthreads();
+  if (tid < kDigits)
+    s.digits[(size_t)tid * s.tiles + tile] = count[tid];
+}
+
+// Exclusive prefix of one value per thread of a workgroup; part: a word per wave.
+__device__ __forceinline__ uint32_t prefix(uint32_t v, uint32_t *part,
+                                           uint32_t &total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t up = v;
+#pragma unroll
+  for (int sh = 1; sh < 64; sh <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_up((int)up, sh);
+    up += lane >= sh ? o : 0u;
+  }
+  __syncthreads(); // (part may be in use)
+  if (lane == 63)
+    part[wave] = up;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kSortThreads / 64; ++w) {
+    before += w < wave ? part[w] : 0u;
+    total += part[w];
+  }
+  return before + up - v;
+}
+
+// A workgroup per digit: entries of the digit in the tiles before each.
+__global__ __launch_bounds__(kSortThreads) void lookup_scan_kernel(Sorted s) {
+  __shared__ uint32_t part[kSortThreads / 64];
+  uint32_t *column = s.digits + (size_t)blockIdx.x * s.tiles;
+  uint32_t before = 0;
+  for (int first = 0; first < s.tiles; first += kSortThreads) {
+    const int at = first + (int)threadIdx.x;
+    const uint32_t v = at < s.tiles ? column[at] : 0u;
+    uint32_t total;
+    const uint32_t run = before + prefix(v, part, total);
+    if (at < s.tiles)
+      column[at] = run;
+    before += total;
+  }
+  if (threadIdx.x == 0)
+    s.digits[(size_t)kDigits * s.tiles + blockIdx.x] = before;
+}
+
+// Ranks of this thread's entries (kPer, 64 apart, the wave's are neighbours) among the
+// entries of the same digit in the tile, and in `local` where a digit's entries begin.
+// place: [waves][kDigits]; afterwards a wave's first place per digit.
+__device__ __forceinline__ void
+rank_tile(const uint64_t (&v)[kPer], int mine, int some, int shift, int bits,
+          uint32_t (*place)[kDigits], uint32_t *part, uint32_t (&rank)[kPer],
+          uint32_t &local) {
+  constexpr int WAVES = kSortThreads / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t mask = (1u << bits) - 1;
+  for (int i = tid; i < WAVES * kDigits; i += kSortThreads)
+    (&place[0][0])[i] = 0u;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t digit = (uint32_t)(v[i] >> 32) >> shift & mask;
+    const bool is = mine + i * 64 < some;
+    uint64_t same = __ballot(is);
+    for (int b = 0; b < bits; ++b) {
+      const bool set = (digit >> b & 1u) != 0u;
+      const uint64_t lanes = __ballot(set);
+      same &= set ? lanes : ~lanes;
+    }
+    // (the first of them counts for all; a wave's atomics come in order)
+    const int leader =
+        same != 0 ? __ffsll((unsigned long long)same) - 1 : lane;
+    uint32_t before = 0;
+    if (is && lane == leader)
+      before = atomicAdd(&place[wave][digit], (uint32_t)__popcll(same));
+    before = (uint32_t)__shfl((int)before, leader);
+    rank[i] = before + (uint32_t)__popcll(same & ((1ull << lane) - 1));
+  }
+  __syncthreads();
+  uint32_t count = 0, total;
+  if (tid < kDigits)
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+      count += place[w][tid];
+  local = prefix(count, part, total);
+  if (tid < kDigits) {
+    uint32_t run = local;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const uint32_t n = place[w][tid];
+      place[w][tid] = run;
+      run += n;
+    }
+  }
+  __syncthreads();
+}
+
+// A tile's entries by digit, those of a digit in the order they came in: put together in
+// LDS first, so that neighbouring threads write neighbouring places.
+__global__ __launch_bounds__(kSortThreads) void
+lookup_scatter_kernel(LookupCall c, Sorted s, Pass p) {
+  __shared__ uint64_t lds[kTile];
+  __shared__ uint32_t place[kSortThreads / 64][kDigits];
+  __shared__ uint32_t part[kSortThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int first = (int)blockIdx.x * kTile;
+  const int some = (int)min((int64_t)kTile, c.entries - first);
+  const int mine = wave * (64 * kPer) + lane;
+  const uint32_t mask = (1u << p.bits) - 1;
+  uint64_t v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    v[i] = pair_at(c, s, p, first + min(mine + i * 64, some - 1));
+  // what is before the digit's entries: of smaller digits, in the tiles before
+  uint32_t offset = 0, all = 0, total;
+  if (tid < kDigits) {
+    offset = s.digits[(size_t)tid * s.tiles + blockIdx.x];
+    all = s.digits[(size_t)kDigits * s.tiles + tid];
+  }
+  uint32_t rank[kPer], local;
+  rank_tile(v, mine, some, p.shift, p.bits, place, part, rank, local);
+  offset += prefix(all, part, total);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const uint32_t digit = (uint32_t)(v[i] >> 32) >> p.shift & mask;
+    if (mine + i * 64 < some)
+      lds[place[wave][digit] + rank[i]] = v[i];
+  }
+  __syncthreads();
+  if (tid < kDigits)
+    place[0][tid] = offset - local; // (modulo 2^32)
+  __syncthreads();
+  uint64_t *out = p.number & 1 ? s.b : s.a;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = i * kSortThreads + tid;
+    if (at < some) {
+      const uint64_t pair = lds[at];
+      const uint32_t to =
+          place[0][(uint32_t)(pair >> 32) >> p.shift & mask] + (uint32_t)at;
+      if (to < (uint64_t)c.entries) {
+        if (p.last) {
+          s.keys[to] = (uint32_t)(pair >> 32);
+          s.perm[to] = (uint32_t)pair;
+        } else {
+          out[to] = pair;
+        }
+      }
+    }
+  }
+}
+
+// All passes of at most a tile's entries, by one workgroup; the others clear the
+// gradient.
+__global__ __launch_bounds__(kSortThreads) void
+lookup_small_sort_kernel(LookupCall c, Sorted s, int bits, int64_t clear) {
+  __shared__ uint64_t lds[kTile];
+  __shared__ uint32_t place[kSortThreads / 64][kDigits];
+  __shared__ uint32_t part[kSortThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (blockIdx.x > 0) {
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * kSortThreads + tid; i < clear;
+         i += (int64_t)(gridDim.x - 1) * kSortThreads)
+      static_cast<uint16_t *>(c.out)[i] = 0;
+    return;
+  }
+  const int some = (int)c.entries;
+  if (some == 0)
+    return;
+  const int mine = wave * (64 * kPer) + lane;
+  uint64_t v[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = min(mine + i * 64, some - 1);
+    v[i] = (uint64_t)key_at(c, e) << 32 | (uint32_t)e;
+  }
+  for (int shift = 0; shift < bits; shift += kBits) {
+    const int now = min(kBits, bits - shift);
+    const uint32_t mask = (1u << now) - 1;
+    uint32_t rank[kPer], local;
+    rank_tile(v, mine, some, shift, now, place, part, rank, local);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (mine + i * 64 < some)
+        lds[place[wave][(uint32_t)(v[i] >> 32) >> shift & mask] + rank[i]] =
+            v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      v[i] = lds[min(mine + i * 64, some - 1)];
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (mine + i * 64 < some) {
+      s.keys[mine + i * 64] = (uint32_t)(v[i] >> 32);
+      s.perm[mine + i * 64] = (uint32_t)v[i];
+    }
+}
+
+// ---- sums of runs ---------------------------------------------------------------
+
+struct Chunks {
+  int64_t length;  // entries of a chunk
+  int64_t count;   // chunks
+  float *ends;     // [count, 2, width]: sums of a chunk's first and last run where
+                   // they do not lie in it
+};
+
+// Lanes that take an entry's row, 16 bytes each (wide rows: in columns of LANES pieces,
+// blockIdx.y).
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void
+lookup_sum_kernel(LookupCall c, Sorted s, Chunks k) {
+  constexpr int PER = 16 / (int)sizeof(T), GROUPS = 256 / LANES, AHEAD = 8;
+  const int lane = threadIdx.x % LANES;
+  const int64_t chunk = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
+  const int64_t e0 = ((int64_t)blockIdx.y * LANES + lane) * PER;
+  if (chunk >= k.count || e0 >= c.width)
+    return;
+  const int64_t begin = chunk * k.length;
+  const int64_t end = min(begin + k.length, c.entries);
+  const uint32_t none = (uint32_t)c.table;
+  const bool vec = c.width % PER == 0;
+  uint32_t now = s.keys[begin];
+  if (now == none)
+    return;
+  bool open = begin > 0 && s.keys[begin - 1] == now; // the run started before
+  float sum[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    sum[i] = 0.f;
+  auto put = [&](bool last) {
+    if (open || last) {
+      float *to = k.ends + (chunk * 2 + (open ? 0 : 1)) * c.width + e0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (vec || e0 + i < c.width)
+          to[i] = sum[i];
+    } else {
+      T *to = static_cast<T *>(c.out) + (int64_t)now * c.width + e0;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (vec || e0 + i < c.width)
+          to[i] = (T)(sum[i] * c.scale);
+    }
+  };
+  for (int64_t at = begin; at < end; at += AHEAD) {
+    T v[AHEAD][PER];
+    uint32_t key[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int64_t e = min(at + j, end - 1);
+      key[j] = s.keys[e];
+      const T *from =
+          static_cast<const T *>(c.rows) + (int64_t)s.perm[e] * c.width + e0;
+      if (vec) {
+        __builtin_memcpy(v[j], __builtin_assume_aligned(from, 16), 16);
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          v[j][i] = e0 + i < c.width ? from[i] : (T)0.f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (at + j >= end)
+        break;
+      if (key[j] != now) {
+        put(false);
+        now = key[j];
+        open = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i)
+          sum[i] = 0.f;
+        if (now == none)
+          return;
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        sum[i] += (float)v[j][i];
+    }
+  }
+  put(end < c.entries && s.keys[end] == now);
+}
+
+// A workgroup per chunk in which a run starts that goes on behind it: the run's parts,
+// dealt to the groups of lanes and put together in the order of the groups.
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void
+lookup_join_kernel(LookupCall c, Sorted s, Chunks k) {
+  constexpr int PER = 16 / (int)sizeof(T), GROUPS = 256 / LANES;
+  __shared__ float part[GROUPS][LANES * PER + 1];
+  __shared__ int64_t after_last;
+  const int64_t chunk = blockIdx.x;
+  const int64_t begin = chunk * k.length;
+  const int64_t end = min(begin + k.length, c.entries);
+  if (end >= c.entries)
+    return;
+  const uint32_t now = s.keys[end - 1];
+  if (now == (uint32_t)c.table || s.keys[end] != now ||
+      (s.keys[begin] == now && begin > 0 && s.keys[begin - 1] == now))
+    return;
+  // chunks behind this one that begin with the run's row
+  if (threadIdx.x == 0) {
+    int64_t lo = chunk + 1, hi = k.count;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) >> 1;
+      if (s.keys[mid * k.length] == now)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    after_last = hi;
+  }
+  __syncthreads();
+  const int64_t stop = after_last;
+  const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  const int64_t e0 = ((int64_t)blockIdx.y * LANES + lane) * PER;
+  float sum[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    sum[i] = 0.f;
+  for (int64_t at = chunk + grp; at < stop; at += GROUPS) {
+    const float *from =
+        k.ends + (at * 2 + (at == chunk ? 1 : 0)) * c.width + e0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (e0 + i < c.width)
+        sum[i] += from[i];
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    part[grp][lane * PER + i] = sum[i];
+  __syncthreads();
+  for (int col = threadIdx.x; col < LANES * PER; col += 256) {
+    const int64_t e = (int64_t)blockIdx.y * LANES * PER + col;
+    if (e >= c.width)
+      continue;
+    float all = 0.f;
+    for (int g = 0; g < GROUPS; ++g)
+      all += part[g][col];
+    static_cast<T *>(c.out)[(int64_t)now * c.width + e] = (T)(all * c.scale);
+  }
+}
+
+int bit_length(uint64_t v) {
+  int n = 0;
+  while (v >> n)
+    ++n;
+  return n;
+}
+
+Chunks chunks_of(int64_t entries) {
+  Chunks k;
+  k.length = std::clamp<int64_t>((entries + 8191) / 8192, 16, 1 << 20);
+  k.count = (entries + k.length - 1) / k.length;
+  k.ends = nullptr;
+  return k;
+}
+
+template <typename T, int LANES>
+void launch_sums(const LookupCall &c, const Sorted &s, const Chunks &k,
+                 hipStream_t stream) {
+  constexpr int PER = 16 / (int)sizeof(T), GROUPS = 256 / LANES;
+  const unsigned columns =
+      (unsigned)((c.width + LANES * PER - 1) / (LANES * PER));
+  lookup_sum_kernel<T, LANES>
+      <<<dim3((unsigned)((k.count + GROUPS - 1) / GROUPS), columns), dim3(256),
+         0, stream>>>(c, s, k);
+  lookup_join_kernel<T, LANES>
+      <<<dim3((unsigned)k.count, columns), dim3(256), 0, stream>>>(c, s, k);
+}
+
+template <typename T>
+hipError_t launch_type(const LookupCall &c, const Sorted &s, const Chunks &k,
+                       hipStream_t stream) {
+  const int64_t pieces = (c.width * (int64_t)sizeof(T) + 15) / 16;
+  if (pieces <= 4)
+    launch_sums<T, 4>(c, s, k, stream);
+  else if (pieces <= 8)
+    launch_sums<T, 8>(c, s, k, stream);
+  else if (pieces <= 16)
+    launch_sums<T, 16>(c, s, k, stream);
+  else if (pieces <= 32)
+    launch_sums<T, 32>(c, s, k, stream);
+  else
+    launch_sums<T, 64>(c, s, k, stream);
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_forward(const LookupCall &c, hipStream_t stream) {
+  const int64_t pieces = (c.width * (int64_t)sizeof(T) + 15) / 16;
+  const int64_t total = pieces * c.entries;
+  const int64_t blocks = std::min<int64_t>((total + 255) / 256, 1 << 16);
+  lookup_kernel<T>
+      <<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(c, pieces, total);
+  return hipGetLastError();
+}
+
+size_t element_size(int dtype) { return dtype == 0 ? 4 : 2; }
+
+} // namespace
+
+hipError_t lookup_forward(const LookupCall &c, int dtype, hipStream_t stream) {
+  if (c.entries == 0 || c.width == 0)
+    return hipSuccess;
+  return dtype == 0   ? launch_forward<float>(c, stream)
+         : dtype == 2 ? launch_forward<_Float16>(c, stream)
+                      : launch_forward<__bf16>(c, stream);
+}
+
+size_t lookup_workspace_bytes(int64_t, int64_t entries, int64_t width) {
+  const Chunks k = chunks_of(entries);
+  const int64_t tiles = (entries + kTile - 1) / kTile;
+  return 2 * lk_align(8 * (size_t)entries) + 2 * lk_align(4 * (size_t)entries) +
+         lk_align(4 * (size_t)kDigits * (size_t)(tiles + 1)) +
+         lk_align(8 * (size_t)k.count * (size_t)width) + 256;
+}
+
+hipError_t lookup_backward(const LookupCall &c, int dtype, void *workspace,
+                           hipStream_t stream) {
+  if (c.table == 0 || c.width == 0)
+    return hipSuccess;
+  char *base = static_cast<char *>(workspace);
+  auto take = [&](size_t bytes) {
+    char *p = base;
+    base += lk_align(bytes);
+    return p;
+  };
+  Sorted s;
+  Chunks k = chunks_of(c.entries);
+  const int64_t tiles = (c.entries + kTile - 1) / kTile;
+  s.tiles = (int)tiles;
+  s.a = reinterpret_cast<uint64_t *>(take(8 * (size_t)c.entries));
+  s.b = reinterpret_cast<uint64_t *>(take(8 * (size_t)c.entries));
+  s.keys = reinterpret_cast<uint32_t *>(take(4 * (size_t)c.entries));
+  s.perm = reinterpret_cast<uint32_t *>(take(4 * (size_t)c.entries));
+  s.digits =
+      reinterpret_cast<uint32_t *>(take(4 * (size_t)kDigits * (tiles + 1)));
+  k.ends = reinterpret_cast<float *>(take(8 * (size_t)k.count * c.width));
+  const int64_t clear =
+      c.table * c.width * (int64_t)(element_size(dtype) / 2);
+  const int bits = bit_length((uint64_t)c.table);
+  if (c.entries <= kTile) {
+    const int64_t fill = std::min<int64_t>(
+        (clear + kSortThreads * 8 - 1) / (kSortThreads * 8), 2048);
+    Sorted one = s;
+    LookupCall some = c;
+    lookup_small_sort_kernel<<<dim3((unsigned)(1 + fill)), dim3(kSortThreads),
+                               0, stream>>>(some, one, bits, clear);
+    if (c.entries == 0)
+      return hipGetLastError();
+  } else {
+    const int passes = (bits + kBits - 1) / kBits;
+    const int each = (bits + passes - 1) / passes;
+    for (int n = 0; n < passes; ++n) {
+      Pass p;
+      p.number = n;
+      p.shift = n * each;
+      p.bits = std::min(each, bits - p.shift);
+      p.last = n == passes - 1;
+      const int64_t fill =
+          n == 0 ? std::min<int64_t>(
+                       (clear + kSortThreads * 8 - 1) / (kSortThreads * 8), 2048)
+                 : 0;
+      lookup_count_kernel<<<dim3((unsigned)std::max<int64_t>(tiles, fill)),
+                            dim3(kSortThreads), 0, stream>>>(
+          c, s, p, n == 0 ? clear : 0);
+      lookup_scan_kernel<<<dim3(kDigits), dim3(kSortThreads), 0, stream>>>(s);
+      lookup_scatter_kernel<<<dim3((unsigned)tiles), dim3(kSortThreads), 0,
+                              stream>>>(c, s, p);
+    }
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return e;
+  return dtype == 0   ? launch_type<float>(c, s, k, stream)
+         : dtype == 2 ? launch_type<_Float16>(c, s, k, stream)
+                      : launch_type<__bf16>(c, s, k, stream);
+}
+
+} // namespace pca
