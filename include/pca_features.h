@@ -67,7 +67,8 @@ typedef struct pca_attention_args {
 /* Scratch of the forward (backward = 0) or the backward call (1); 0: sizes not
  * supported. */
 size_t pca_attention_workspace_bytes(int64_t nq, int64_t nk, int32_t hq,
-                                     int32_t hk, int32_t d, int backward);
+                                     int32_t hk, int32_t d, int32_t dtype,
+                                     int backward);
 
 /* out: [nq, hq, d] dense.  lse: [hq, nq] fp32 for the backward pass, or NULL. */
 int pca_attention_forward(const pca_attention_args *args, void *out, float *lse,

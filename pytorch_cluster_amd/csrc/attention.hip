@@ -174,17 +174,18 @@ hipError_t join_sum(const AttentionCall &c, const float *part, int64_t stride,
 
 } // namespace
 
-AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk) {
+AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
+                             int dtype, int d) {
   const int64_t rows_q = nq * (hq / hk);
   const int64_t owned = pass == 2 ? nk : rows_q;
   const int64_t looped = pass == 2 ? rows_q : nk;
   AttentionPlan p;
-  const int64_t wide =
-      (owned + attn::kWideRows - 1) / attn::kWideRows * hk;
+  const int rows = wide_rows(pass, dtype == 0 ? 4 : 2, d);
+  const int64_t wide = (owned + rows - 1) / rows * hk;
   p.wide = wide >= 256;
   if (!p.wide) {
     const int64_t few =
-        std::max<int64_t>(1, (owned + attn::kFewRows - 1) / attn::kFewRows * hk);
+        std::max<int64_t>(1, (owned + kFewRows - 1) / kFewRows * hk);
     const int64_t most = (looped + 255) / 256;
     p.splits = (int)std::clamp<int64_t>(1024 / few, 1,
                                         std::clamp<int64_t>(most, 1, 256));
@@ -192,8 +193,9 @@ AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk) {
   return p;
 }
 
-static size_t part_bytes(int pass, int splits, int64_t nq, int64_t nk, int hq,
-                         int hk, int d) {
+static size_t part_bytes(int pass, int64_t nq, int64_t nk, int hq, int hk,
+                         int dtype, int d) {
+  const int splits = attention_plan(pass, nq, nk, hq, hk, dtype, d).splits;
   if (splits <= 1)
     return 0;
   const int64_t one = pass == 2 ? 2 * nk * hk * d : nq * hq * d;
@@ -204,20 +206,17 @@ static size_t part_bytes(int pass, int splits, int64_t nq, int64_t nk, int hq,
 }
 
 size_t attention_workspace_bytes(int pass, int64_t nq, int64_t nk, int hq,
-                                 int hk, int d) {
+                                 int hk, int dtype, int d) {
   if (pass == 0)
-    return 256 + part_bytes(0, attention_plan(0, nq, nk, hq, hk).splits, nq, nk,
-                            hq, hk, d);
+    return 256 + part_bytes(0, nq, nk, hq, hk, dtype, d);
   return attn_align(sizeof(float) * (size_t)(nq * hq)) + 256 +
-         std::max(part_bytes(1, attention_plan(1, nq, nk, hq, hk).splits, nq, nk,
-                             hq, hk, d),
-                  part_bytes(2, attention_plan(2, nq, nk, hq, hk).splits, nq, nk,
-                             hq, hk, d));
+         std::max(part_bytes(1, nq, nk, hq, hk, dtype, d),
+                  part_bytes(2, nq, nk, hq, hk, dtype, d));
 }
 
 hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
                              hipStream_t stream) {
-  const AttentionPlan p = attention_plan(0, c.nq, c.nk, c.hq, c.hk);
+  const AttentionPlan p = attention_plan(0, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
   c.splits = p.splits;
   c.part = static_cast<float *>(workspace);
   c.part_ml = c.part + attn_align(sizeof(float) * (size_t)p.splits * c.nq *
@@ -237,7 +236,7 @@ hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
   c.delta = static_cast<float *>(workspace);
   c.part = c.delta +
            attn_align(sizeof(float) * (size_t)c.nq * c.hq) / sizeof(float);
-  const AttentionPlan pq = attention_plan(1, c.nq, c.nk, c.hq, c.hk);
+  const AttentionPlan pq = attention_plan(1, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
   c.splits = pq.splits;
   hipError_t e = launcher(dtype, c.d)(c, 1, pq.wide, stream);
   if (e == hipSuccess && c.splits > 1 && c.nq > 0) {
@@ -246,7 +245,7 @@ hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
   }
   if (e != hipSuccess)
     return e;
-  const AttentionPlan pk = attention_plan(2, c.nq, c.nk, c.hq, c.hk);
+  const AttentionPlan pk = attention_plan(2, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
   c.splits = pk.splits;
   e = launcher(dtype, c.d)(c, 2, pk.wide, stream);
   if (e == hipSuccess && c.splits > 1 && c.nk > 0) {

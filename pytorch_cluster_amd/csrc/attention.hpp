@@ -65,11 +65,18 @@ PCA_ATTENTION_DECLARE(f16);
 PCA_ATTENTION_DECLARE(bf16);
 #undef PCA_ATTENTION_DECLARE
 
-constexpr int kAttentionMaxD = 128;
+// Owned rows of a workgroup: of the kernels whose waves own rows of their own, and of
+// those for few rows.  Two blocks of 16 columns per wave share every left operand; where
+// the sums of both do not fit the registers of two waves per SIMD it is one.
+constexpr int kFewRows = 16;
+constexpr int wide_rows(int pass, int size, int width) {
+  return width > 64 && (pass == 2 || (pass == 1 && size == 4)) ? 64 : 128;
+}
 
-AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk);
+AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
+                             int dtype, int d);
 size_t attention_workspace_bytes(int pass, int64_t nq, int64_t nk, int hq,
-                                 int hk, int d);
+                                 int hk, int dtype, int d);
 // workspace: of attention_workspace_bytes(0, ...) / (1, ...)
 hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
                              hipStream_t stream);

@@ -82,10 +82,15 @@ template <typename T, int DP> struct Shape {
   static constexpr int CH = DP / PER;          // 16-byte pieces of a row
   static constexpr int KS = CH / 4;            // steps of a product over d
   static constexpr int DB = DP / 16;           // 16-wide blocks over d
-  static constexpr int PITCH = DP * SZ + 16;   // bytes of a row in LDS: 16 rows
-                                               // start on 16 different banks
+  static constexpr int BYTES = DP * SZ;        // of a row in LDS
   static constexpr int KF = SZ == 2 ? 32 : 16; // rows of a step over rows
   static constexpr int FB = KF / 16;           // ... in blocks
+  // A tile's rows lie in LDS one after the other, as the loads that bypass the
+  // registers leave them.  Piece p of row r is kept at place p ^ turn(r): the same
+  // piece of 16 neighbouring rows then lies on 64 different banks.
+  __device__ __forceinline__ static int turn(int row) {
+    return CH >= 16 ? row & 15 : (row / (16 / CH)) & (CH - 1);
+  }
 };
 
 // 16 bytes of row `row` at piece `piece`; zeros beyond d.
@@ -109,49 +114,127 @@ __device__ __forceinline__ u32x4 load_piece(const HeadRows &x, int64_t row,
   return r;
 }
 
-// ROWS rows of [begin, end) on their way from memory to LDS.  A row stands for
-// (row / group, head0 + row % group).
-template <typename T, int DP, int ROWS> struct Stage {
-  using S = Shape<T, DP>;
-  static constexpr int N = ROWS * S::CH / kThreads;
-  static_assert(ROWS * S::CH % kThreads == 0, "tile does not fill the threads");
-  u32x4 v[N];
+// What rows behind the end of a span are read from.
+static __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
-  __device__ __forceinline__ void load(const HeadRows &x, int begin, int end,
-                                       int group, int head0, int d) {
+// Loads that go from memory to LDS without registers: lane l's 16 (4) bytes to `lds` +
+// 16 l (4 l).  Nothing waits for them but arrive().
+__device__ __forceinline__ void request16(const void *from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\t"
+               "s_nop 0\n\t"
+               "global_load_lds_dwordx4 %0, off"
+               :
+               : "v"(from), "s"(lds)
+               : "memory");
+}
+__device__ __forceinline__ void request16(const void *base, uint32_t offset,
+                                          uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\t"
+               "s_nop 0\n\t"
+               "global_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(offset), "s"(base), "s"(lds)
+               : "memory");
+}
+__device__ __forceinline__ void request4(const void *from, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %1\n\t"
+               "s_nop 0\n\t"
+               "global_load_lds_dword %0, off"
+               :
+               : "v"(from), "s"(lds)
+               : "memory");
+}
+// Everything this wave has requested is in LDS; then everything the others have.
+__device__ __forceinline__ void arrive() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  return (uint32_t)(uintptr_t)p; // (the low half of a generic address)
+}
+
+// Rows of looped tiles of one tensor on their way to LDS: ROWS rows of [begin, end),
+// zeros behind the end.  A row stands for (row / group, head0 + row % group).  Pieces
+// beyond d are left alone: the caller has cleared them.
+template <typename T, int DP, int ROWS> struct Requests {
+  using S = Shape<T, DP>;
+  static constexpr int N = ROWS * S::CH / kThreads;      // per thread
+  static constexpr int STEP = kThreads / S::CH;          // rows between them
+  static constexpr int LANES = STEP % 16 == 0 ? 1 : 2;   // places turned alike
+  static_assert(ROWS * S::CH % kThreads == 0, "tile does not fill the threads");
+  const HeadRows &x;
+  int d, wave;
+  uint32_t offset[LANES]; // bytes of this thread's first pieces from a tile's row
+
+  __device__ __forceinline__ Requests(const HeadRows &rows, int width)
+      : x(rows), d(width) {
+    wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = threadIdx.x + i * kThreads;
-      const int row = begin + c / S::CH;
-      v[i] = u32x4{0, 0, 0, 0};
-      if (row < end) {
-        const int r = group == 1 ? row : row / group;
-        v[i] = load_piece<T, DP>(x, r, head0 + row - r * group, c % S::CH, d);
+    for (int l = 0; l < LANES; ++l)
+      offset[l] = (uint32_t)((threadIdx.x / S::CH) * x.row * S::SZ) +
+                  piece(threadIdx.x / S::CH + l * STEP) * 16;
+  }
+  __device__ __forceinline__ static int piece(int row) {
+    return threadIdx.x % S::CH ^ S::turn(row);
+  }
+  __device__ __forceinline__ void operator()(int begin, int end, int group,
+                                             int head0, char *tile) const {
+    const uint32_t lds = lds_address(tile) + wave * 1024;
+    if (x.vec && group == 1 && begin + ROWS <= end) {
+      const char *base = static_cast<const char *>(x.data) +
+                         ((int64_t)begin * x.row + (int64_t)head0 * x.head) *
+                             S::SZ;
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (piece(threadIdx.x / S::CH + e * STEP) * S::PER < d)
+          request16(base + (int64_t)(e * STEP) * x.row * S::SZ,
+                    offset[e % LANES], lds + kWaves * e * 1024);
+      return;
+    }
+#pragma unroll 1
+    for (int e = 0; e < N; ++e) {
+      const int row = threadIdx.x / S::CH + e * STEP;
+      const int at = begin + row;
+      const int r = group == 1 ? at : at / group;
+      const int head = group == 1 ? head0 : head0 + at - r * group;
+      const int p = piece(row);
+      if (x.vec) {
+        const T *from = static_cast<const T *>(x.data) + (int64_t)r * x.row +
+                        (int64_t)head * x.head + p * S::PER;
+        if (p * S::PER < d)
+          request16(at < end ? (const void *)from : (const void *)kZeros,
+                    lds + kWaves * e * 1024);
+      } else {
+        u32x4 v = {0, 0, 0, 0};
+        if (at < end)
+          v = load_piece<T, DP>(x, r, head, p, d);
+        *reinterpret_cast<u32x4 *>(tile + (threadIdx.x + e * kThreads) * 16) =
+            v;
       }
     }
   }
-  __device__ __forceinline__ void store(char *tile) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int c = threadIdx.x + i * kThreads;
-      *reinterpret_cast<u32x4 *>(tile + (c / S::CH) * S::PITCH +
-                                 (c % S::CH) * 16) = v[i];
-    }
-  }
 };
+
+// Clears what requests leave alone.
+template <int BYTES> __device__ __forceinline__ void clear_lds(char *p) {
+  for (int i = threadIdx.x * 16; i < BYTES; i += kThreads * 16)
+    *reinterpret_cast<u32x4 *>(p + i) = u32x4{0, 0, 0, 0};
+  __syncthreads();
+}
 
 // Left operand with the tile's rows as its rows: row block `block`, step `ks` of d.
 template <typename T, int DP>
 __device__ __forceinline__ u32x4 rows_operand(const char *tile, int block,
                                               int ks) {
-  const int lane = threadIdx.x & 63;
+  using S = Shape<T, DP>;
+  const int lane = threadIdx.x & 63, i = lane & 15;
   return *reinterpret_cast<const u32x4 *>(
-      tile + (block * 16 + (lane & 15)) * Shape<T, DP>::PITCH + ks * 64 +
-      (lane >> 4) * 16);
+      tile + (block * 16 + i) * S::BYTES +
+      ((lane >> 4 ^ S::turn(i)) ^ ks * 4) * 16);
 }
 
-// Left operand with d as its rows (16 from d0) and the tile's rows from `row0` as the
-// contraction, in the order described above.
+// Left operand with d as its rows (16 of block `db`) and the tile's rows from `row0` (a
+// multiple of 16) as the contraction, in the order described above.
 template <typename T, int DP>
 __device__ __forceinline__ u32x4 turned_operand(const char *tile, int row0,
                                                 int db) {
@@ -159,21 +242,25 @@ __device__ __forceinline__ u32x4 turned_operand(const char *tile, int row0,
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
   if constexpr (S::SZ == 4) {
     u32x4 r;
-    const char *p = tile + (row0 + g * 4) * S::PITCH + (db * 16 + i) * 4;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      r[c] = *reinterpret_cast<const uint32_t *>(p + c * S::PITCH);
+    for (int c = 0; c < 4; ++c) {
+      const int row = g * 4 + c;
+      r[c] = *reinterpret_cast<const uint32_t *>(
+          tile + (row0 + row) * S::BYTES +
+          ((i >> 2 ^ S::turn(row)) ^ db * 4) * 16 + (i & 3) * 4);
+    }
     return r;
   } else {
     // lane i of a group of 16 names 4 elements of row i / 4 and gets column i of
     // the 4 x 16 elements that the group names
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const char *p =
-        tile + (row0 + g * 4 + (i >> 2)) * S::PITCH + (db * 16 + (i & 3) * 4) * 2;
+    const int row = g * 4 + (i >> 2);
+    const char *p = tile + (row0 + row) * S::BYTES +
+                    (((i & 3) >> 1 ^ S::turn(row)) ^ db * 2) * 16 + (i & 1) * 8;
     const s16x4 lo =
         __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_s16x4 *)(p + 16 * S::PITCH));
+        (lds_s16x4 *)(p + 16 * S::BYTES));
     const u32x2 a = __builtin_bit_cast(u32x2, lo);
     const u32x2 b = __builtin_bit_cast(u32x2, hi);
     return u32x4{a[0], a[1], b[0], b[1]};
@@ -330,10 +417,16 @@ template <int ROWS> struct Walk {
         ++span;
   }
   __device__ __forceinline__ bool there() const { return at < stop; }
-  __device__ __forceinline__ int begin() const {
-    return s.begin[span] + (at - s.first[span]) * tile;
+  __device__ __forceinline__ int first() const {
+    return __builtin_amdgcn_readfirstlane(s.begin[span]);
   }
-  __device__ __forceinline__ int end() const { return s.end[span]; }
+  __device__ __forceinline__ int begin() const {
+    return __builtin_amdgcn_readfirstlane(s.begin[span] +
+                                          (at - s.first[span]) * tile);
+  }
+  __device__ __forceinline__ int end() const {
+    return __builtin_amdgcn_readfirstlane(s.end[span]);
+  }
   __device__ __forceinline__ void next() {
     ++at;
     settle();
@@ -395,37 +488,96 @@ __device__ __forceinline__ Column query_column(const AttentionCall &c, int row,
   return r;
 }
 
-// Scores of a block in units of log 2, from the products; `key`: positions of the four
-// looped rows, `slope` per row.  Leaves 1 - tanh^2 in `flat` if asked for.
-template <typename T, bool FLAT>
-__device__ __forceinline__ void
-scores(f32x4 &s, const AttentionCall &c, const float (&p)[3],
-       const f32x4 (&other)[3], f32x4 slope, f32x4 *flat) {
+// Scores in units of log 2, from the products of RB x NB blocks.  Leaves 1 - tanh^2 in
+// `flat` if asked for.
+template <typename T, bool FLAT, int RB, int NB>
+__device__ __forceinline__ void cap_scores(f32x4 (&s)[RB][NB],
+                                           const AttentionCall &c,
+                                           f32x4 (*flat)[NB]) {
   if (c.cap > 0.f) {
     const float in = c.scale / c.cap * (2.f * kLog2e), out = c.cap * kLog2e;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float t = tanh_of<T>(s[r] * in);
-      s[r] = t * out;
-      if (FLAT)
-        (*flat)[r] = 1.f - t * t;
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float t = tanh_of<T>(s[rb][b][r] * in);
+          s[rb][b][r] = t * out;
+          if constexpr (FLAT)
+            flat[rb][b][r] = fmaf(-t, t, 1.f);
+        }
+  } else {
+    const float in = c.scale * kLog2e;
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        s[rb][b] *= in;
+  }
+}
+
+// Takes slope times distance off: p of the columns, `pos` of the looped rows.
+__device__ __forceinline__ float far_by(const float (&p)[3], float x) {
+  return fabsf(p[0] - x);
+}
+__device__ __forceinline__ float far_by(const float (&p)[3], float x, float y,
+                                        float z) {
+  const float a = p[0] - x, b = p[1] - y, e = p[2] - z;
+  return __builtin_amdgcn_sqrtf(fmaf(e, e, fmaf(b, b, a * a)));
+}
+
+// Positions of rows [begin, end) to LDS, axis by axis (the third of two stays as it is:
+// cleared).
+template <int KT>
+__device__ __forceinline__ void request_positions(const float *pos, int begin,
+                                                  int end, int axes,
+                                                  float (*lds)[KT]) {
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave * 64 < KT) {
+    const int row = begin + wave * 64 + lane;
+    for (int a = 0; a < axes; ++a)
+      if (KT >= 64 || lane < KT)
+        request4(row < end ? (const void *)(pos + (int64_t)row * axes + a)
+                           : (const void *)kZeros,
+                 lds_address(&lds[a][wave * 64]));
+  }
+}
+
+// The four looped rows of a block that a lane has scores of: `at`, at + 1, ...
+template <int RB, int NB, int KT>
+__device__ __forceinline__ void take_distance(f32x4 (&s)[RB][NB],
+                                              const AttentionCall &c,
+                                              const Column (&col)[RB],
+                                              const float (&pos)[3][KT],
+                                              int part) {
+  const int g = (threadIdx.x & 63) >> 4;
+  if (c.axes == 1) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int at = part + b * 16 + g * 4;
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(&pos[0][at]);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[rb][b][r] =
+              fmaf(-col[rb].slope, far_by(col[rb].p, x[r]), s[rb][b][r]);
     }
   } else {
-    s *= c.scale * kLog2e;
-  }
-  if (c.slope) {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float x = p[0] - other[0][r];
-      float d2 = x * x;
-      if (c.axes > 1) {
-        const float y = p[1] - other[1][r], z = p[2] - other[2][r];
-        d2 = fmaf(z, z, fmaf(y, y, d2));
-        d2 = __builtin_amdgcn_sqrtf(d2);
-      } else {
-        d2 = fabsf(x);
-      }
-      s[r] = fmaf(-slope[r], d2, s[r]);
+    for (int b = 0; b < NB; ++b) {
+      const int at = part + b * 16 + g * 4;
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(&pos[0][at]);
+      const f32x4 y = *reinterpret_cast<const f32x4 *>(&pos[1][at]);
+      const f32x4 z = *reinterpret_cast<const f32x4 *>(&pos[2][at]);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          s[rb][b][r] = fmaf(-col[rb].slope,
+                             far_by(col[rb].p, x[r], y[r], z[r]), s[rb][b][r]);
     }
   }
 }
@@ -435,16 +587,15 @@ scores(f32x4 &s, const AttentionCall &c, const float (&p)[3],
 // Rows of a wave's columns: RB blocks of 16.  WK waves share the same columns and
 // divide every tile among them (few rows); the others own columns of their own.
 template <typename T, int DP, int RB, int WK>
-__global__ __launch_bounds__(kThreads) void
+__global__ __launch_bounds__(kThreads, 2) void
 attention_forward_kernel(AttentionCall c) {
   using S = Shape<T, DP>;
   constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
   constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
   constexpr int KB = KW / 16;
-  constexpr int TILE = KT * S::PITCH;
-  __shared__ __attribute__((aligned(16))) char lds_tiles[2 * TILE];
-  char *const lds_k = lds_tiles, *const lds_v = lds_tiles + TILE;
-  __shared__ __attribute__((aligned(16))) float lds_pos[3][KT];
+  constexpr int TILE = KT * S::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds_tiles[4 * TILE];
+  __shared__ __attribute__((aligned(16))) float lds_pos[2][3][KT];
   __shared__ float lds_ml[kWaves][16][2];
   __shared__ Spans<ROWS> spans;
 
@@ -478,37 +629,33 @@ attention_forward_kernel(AttentionCall c) {
     l[rb] = 0.f;
   }
 
-  Stage<T, DP, KT> stage_k, stage_v;
-  float stage_pos[3];
-  auto fetch = [&](int begin, int end) {
-    stage_k.load(c.k, begin, end, 1, place.head, c.d);
-    stage_v.load(c.v, begin, end, 1, place.head, c.d);
-    if (c.slope && threadIdx.x < KT) {
-      stage_pos[0] = stage_pos[1] = stage_pos[2] = 0.f;
-      const int row = begin + threadIdx.x;
-      if (row < end)
-        load_position(stage_pos, c.pos_k, row, c.axes);
-    }
+  const Requests<T, DP, KT> request_k(c.k, c.d), request_v(c.v, c.d);
+  // Two buffers: while a tile is worked on, the next one is on its way.
+  auto request = [&](int begin, int end, int buffer) {
+    char *tile = lds_tiles + buffer * 2 * TILE;
+    request_k(begin, end, 1, place.head, tile);
+    request_v(begin, end, 1, place.head, tile + TILE);
+    if (c.slope)
+      request_positions<KT>(c.pos_k, begin, end, c.axes, lds_pos[buffer]);
   };
+  if (c.axes == 2)
+    clear_lds<sizeof(lds_pos)>(reinterpret_cast<char *>(lds_pos));
+  if (c.d < DP)
+    clear_lds<4 * TILE>(lds_tiles);
 
   Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  int buffer = 0;
   if (walk.there())
-    fetch(walk.begin(), walk.end());
-  while (walk.there()) {
-    const int begin = walk.begin(), end = walk.end();
-    const int2 span = make_int2(spans.begin[walk.span], end);
-    __syncthreads();
-    stage_k.store(lds_k);
-    stage_v.store(lds_v);
-    if (c.slope && threadIdx.x < KT) {
-#pragma unroll
-      for (int a = 0; a < 3; ++a)
-        lds_pos[a][threadIdx.x] = stage_pos[a];
-    }
-    __syncthreads();
+    request(walk.begin(), walk.end(), 0);
+  for (; walk.there(); buffer ^= 1) {
+    const int2 span = make_int2(walk.first(), walk.end());
+    const int begin = walk.begin(), end = span.y;
+    arrive();
     walk.next();
     if (walk.there())
-      fetch(walk.begin(), walk.end());
+      request(walk.begin(), walk.end(), buffer ^ 1);
+    const char *lds_k = lds_tiles + buffer * 2 * TILE + part * S::BYTES;
+    const char *lds_v = lds_k + TILE;
 
     bool in[RB];
     bool any = false, all = true;
@@ -533,41 +680,34 @@ attention_forward_kernel(AttentionCall c) {
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int ks = 0; ks < S::KS; ++ks) {
-        const u32x4 a =
-            rows_operand<T, DP>(lds_k + part * S::PITCH, kb, ks);
+        const u32x4 a = rows_operand<T, DP>(lds_k, kb, ks);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
           mma<T>(s[rb][kb], a, q[rb][ks]);
       }
 
-    float top[RB];
+    cap_scores<T, false, RB, KB>(s, c, nullptr);
+    if (c.slope)
+      take_distance<RB, KB>(s, c, col, lds_pos[buffer], part);
+    if (cut || mixed) {
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-      top[rb] = -__builtin_inff();
+      for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb) {
-      f32x4 pos[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
-      const int at = part + kb * 16 + g * 4;
-      if (c.slope) {
-#pragma unroll
-        for (int a = 0; a < 3; ++a)
-          pos[a] = *reinterpret_cast<const f32x4 *>(&lds_pos[a][at]);
-      }
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb) {
-        const float sl = col[rb].slope;
-        scores<T, false>(s[rb][kb], c, col[rb].p, pos, f32x4{sl, sl, sl, sl},
-                         nullptr);
-        if (cut || mixed) {
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (!in[rb] || begin + at + r >= end)
+            if (!in[rb] || begin + part + kb * 16 + g * 4 + r >= end)
               s[rb][kb][r] = -__builtin_inff();
-        }
+    }
+    float top[RB];
+#pragma unroll
+    for (int rb = 0; rb < RB; ++rb) {
+      top[rb] = s[rb][0][0];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
           top[rb] = fmaxf(top[rb], s[rb][kb][r]);
-      }
     }
 
     // The maximum that is subtracted moves only when it would grow by more than 8
@@ -613,7 +753,7 @@ attention_forward_kernel(AttentionCall c) {
         p[rb] = block_operand<T>(&s[rb][f * S::FB]);
 #pragma unroll
       for (int db = 0; db < S::DB; ++db) {
-        const u32x4 a = turned_operand<T, DP>(lds_v, part + f * S::KF, db);
+        const u32x4 a = turned_operand<T, DP>(lds_v, f * S::KF, db);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           if (mixed) {
@@ -638,7 +778,7 @@ attention_forward_kernel(AttentionCall c) {
     // the waves' shares of the same 16 columns: one maximum, then sums in the order
     // of the waves
     static_assert(RB == 1 && WQ == 1, "one block of columns");
-    static_assert(kWaves * 16 * (DP + 4) * 4 <= 2 * TILE, "sums do not fit");
+    static_assert(kWaves * 16 * (DP + 4) * 4 <= 4 * TILE, "sums do not fit");
     auto lds_acc = reinterpret_cast<float(*)[16][DP + 4]>(lds_tiles);
     if (g == 0) {
       lds_ml[wave][i][0] = m[0];
@@ -800,15 +940,14 @@ store_columns(const Sums<T, DP, RB> &acc, int rb, void *out, float *part,
 // dq of the rows that a workgroup owns, looping over keys; writes delta for the kernel
 // of dk and dv.
 template <typename T, int DP, int RB, int WK>
-__global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttentionCall c) {
+__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall c) {
   using S = Shape<T, DP>;
   constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
   constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
   constexpr int KB = KW / 16;
-  constexpr int TILE = KT * S::PITCH;
-  __shared__ __attribute__((aligned(16))) char lds_tiles[2 * TILE];
-  char *const lds_k = lds_tiles, *const lds_v = lds_tiles + TILE;
-  __shared__ __attribute__((aligned(16))) float lds_pos[3][KT];
+  constexpr int TILE = KT * S::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds_tiles[4 * TILE];
+  __shared__ __attribute__((aligned(16))) float lds_pos[2][3][KT];
   __shared__ Spans<ROWS> spans;
 
   const int group = c.hq / c.hk, rows = c.nq * group;
@@ -866,37 +1005,33 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttentionCall c)
       acc[db][rb] = f32x4{0, 0, 0, 0};
   }
 
-  Stage<T, DP, KT> stage_k, stage_v;
-  float stage_pos[3];
-  auto fetch = [&](int begin, int end) {
-    stage_k.load(c.k, begin, end, 1, place.head, c.d);
-    stage_v.load(c.v, begin, end, 1, place.head, c.d);
-    if (c.slope && threadIdx.x < KT) {
-      stage_pos[0] = stage_pos[1] = stage_pos[2] = 0.f;
-      const int row = begin + threadIdx.x;
-      if (row < end)
-        load_position(stage_pos, c.pos_k, row, c.axes);
-    }
+  const Requests<T, DP, KT> request_k(c.k, c.d), request_v(c.v, c.d);
+  // Two buffers: while a tile is worked on, the next one is on its way.
+  auto request = [&](int begin, int end, int buffer) {
+    char *tile = lds_tiles + buffer * 2 * TILE;
+    request_k(begin, end, 1, place.head, tile);
+    request_v(begin, end, 1, place.head, tile + TILE);
+    if (c.slope)
+      request_positions<KT>(c.pos_k, begin, end, c.axes, lds_pos[buffer]);
   };
+  if (c.axes == 2)
+    clear_lds<sizeof(lds_pos)>(reinterpret_cast<char *>(lds_pos));
+  if (c.d < DP)
+    clear_lds<4 * TILE>(lds_tiles);
 
   Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  int buffer = 0;
   if (walk.there())
-    fetch(walk.begin(), walk.end());
-  while (walk.there()) {
-    const int begin = walk.begin(), end = walk.end();
-    const int2 span = make_int2(spans.begin[walk.span], end);
-    __syncthreads();
-    stage_k.store(lds_k);
-    stage_v.store(lds_v);
-    if (c.slope && threadIdx.x < KT) {
-#pragma unroll
-      for (int a = 0; a < 3; ++a)
-        lds_pos[a][threadIdx.x] = stage_pos[a];
-    }
-    __syncthreads();
+    request(walk.begin(), walk.end(), 0);
+  for (; walk.there(); buffer ^= 1) {
+    const int2 span = make_int2(walk.first(), walk.end());
+    const int begin = walk.begin(), end = span.y;
+    arrive();
     walk.next();
     if (walk.there())
-      fetch(walk.begin(), walk.end());
+      request(walk.begin(), walk.end(), buffer ^ 1);
+    const char *lds_k = lds_tiles + buffer * 2 * TILE + part * S::BYTES;
+    const char *lds_v = lds_k + TILE;
 
     bool in[RB];
     bool any = false, all = true;
@@ -913,59 +1048,65 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttentionCall c)
 
 #pragma unroll
     for (int f = 0; f < KB / S::FB; ++f) {
-      f32x4 ds[RB][S::FB];
-      float top[RB];
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-        top[rb] = 0.f;
+      f32x4 s[RB][S::FB], ds[RB][S::FB], flat[RB][S::FB];
 #pragma unroll
       for (int b = 0; b < S::FB; ++b) {
-        const int kb = f * S::FB + b;
-        f32x4 s[RB], dp[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
-          s[rb] = dp[rb] = f32x4{0, 0, 0, 0};
+          s[rb][b] = ds[rb][b] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
-          const u32x4 a = rows_operand<T, DP>(lds_k + part * S::PITCH, kb, ks);
-          const u32x4 b2 = rows_operand<T, DP>(lds_v + part * S::PITCH, kb, ks);
+          const u32x4 ak = rows_operand<T, DP>(lds_k, f * S::FB + b, ks);
+          const u32x4 av = rows_operand<T, DP>(lds_v, f * S::FB + b, ks);
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
-            mma<T>(s[rb], a, q[rb][ks]);
-            mma<T>(dp[rb], b2, dout[rb][ks]);
-          }
-        }
-        f32x4 pos[3] = {{0, 0, 0, 0}, {0, 0, 0, 0}, {0, 0, 0, 0}};
-        const int at = part + kb * 16 + g * 4;
-        if (c.slope) {
-#pragma unroll
-          for (int a = 0; a < 3; ++a)
-            pos[a] = *reinterpret_cast<const f32x4 *>(&lds_pos[a][at]);
-        }
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          const float sl = col[rb].slope;
-          f32x4 flat;
-          scores<T, true>(s[rb], c, col[rb].p, pos, f32x4{sl, sl, sl, sl},
-                          &flat);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = __builtin_amdgcn_exp2f(s[rb][r] - lse[rb]) *
-                      (dp[rb][r] - delta[rb]);
-            if (c.cap > 0.f)
-              v *= flat[r];
-            if ((cut || mixed) && (!in[rb] || begin + at + r >= end))
-              v = 0.f;
-            ds[rb][b][r] = v;
-            top[rb] = fmaxf(top[rb], fabsf(v));
+            mma<T>(s[rb][b], ak, q[rb][ks]);
+            mma<T>(ds[rb][b], av, dout[rb][ks]);
           }
         }
       }
-      if constexpr (Range<T>::on) {
-        bool moves = false;
+      cap_scores<T, true, RB, S::FB>(s, c, flat);
+      if (c.slope)
+        take_distance<RB, S::FB>(s, c, col, lds_pos[buffer], part + f * S::KF);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int b = 0; b < S::FB; ++b)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            ds[rb][b][r] = __builtin_amdgcn_exp2f(s[rb][b][r] - lse[rb]) *
+                           (ds[rb][b][r] - delta[rb]);
+      if (c.cap > 0.f) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+            ds[rb][b] *= flat[rb][b];
+      }
+      if (cut || mixed) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!in[rb] ||
+                  begin + part + f * S::KF + b * 16 + g * 4 + r >= end)
+                ds[rb][b][r] = 0.f;
+      }
+      if constexpr (Range<T>::on) {
+        float top[RB];
+        bool moves = false;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          top[rb] = 0.f;
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              top[rb] = fmaxf(top[rb], fabsf(ds[rb][b][r]));
           moves |= range[rb].moves(top[rb]);
+        }
         if (__ballot(moves) != 0) {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
@@ -987,7 +1128,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttentionCall c)
         p[rb] = block_operand<T>(ds[rb]);
 #pragma unroll
       for (int db = 0; db < S::DB; ++db) {
-        const u32x4 a = turned_operand<T, DP>(lds_k, part + f * S::KF, db);
+        const u32x4 a = turned_operand<T, DP>(lds_k, f * S::KF, db);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           if (mixed) {
@@ -1010,7 +1151,7 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttentionCall c)
     for (int db = 0; db < S::DB; ++db)
       acc[db][rb] *= 1.f / range[rb].factor;
   if constexpr (WK > 1) {
-    static_assert(kWaves * 16 * (DP + 4) * 4 <= 2 * TILE, "sums do not fit");
+    static_assert(kWaves * 16 * (DP + 4) * 4 <= 4 * TILE, "sums do not fit");
     auto lds_acc = reinterpret_cast<float(*)[16][DP + 4]>(lds_tiles);
     join_waves<T, DP, RB, WK>(acc, lds_acc);
   }
@@ -1028,17 +1169,16 @@ __global__ __launch_bounds__(kThreads) void attention_dq_kernel(AttentionCall c)
 
 // dk and dv of the keys that a workgroup owns, looping over (query, head) rows.
 template <typename T, int DP, int RB, int WK>
-__global__ __launch_bounds__(kThreads) void
+__global__ __launch_bounds__(kThreads, 2) void
 attention_dkv_kernel(AttentionCall c) {
   using S = Shape<T, DP>;
   constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
   constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
   constexpr int KB = KW / 16;
-  constexpr int TILE = KT * S::PITCH;
-  __shared__ __attribute__((aligned(16))) char lds_tiles[2 * TILE];
-  char *const lds_q = lds_tiles, *const lds_do = lds_tiles + TILE;
-  // per looped row: position, slope (times log2 e), lse, delta
-  __shared__ __attribute__((aligned(16))) float lds_row[6][KT];
+  constexpr int TILE = KT * S::BYTES;
+  __shared__ __attribute__((aligned(16))) char lds_tiles[4 * TILE];
+  // per looped row: position, slope, lse, delta
+  __shared__ __attribute__((aligned(16))) float lds_row[2][6][KT];
   __shared__ Spans<ROWS> spans;
 
   const int group = c.hq / c.hk;
@@ -1078,50 +1218,48 @@ attention_dkv_kernel(AttentionCall c) {
       acc_k[db][rb] = acc_v[db][rb] = f32x4{0, 0, 0, 0};
   }
 
-  Stage<T, DP, KT> stage_q, stage_do;
-  float stage_row[6];
-  auto fetch = [&](int begin, int end) {
-    stage_q.load(c.q, begin, end, group, head0, c.d);
-    stage_do.load(c.dout, begin, end, group, head0, c.d);
-    if (threadIdx.x < KT) {
-#pragma unroll
-      for (int a = 0; a < 6; ++a)
-        stage_row[a] = 0.f;
-      const int row = begin + threadIdx.x;
-      if (row < end) {
-        const int query = row / group, head = head0 + row % group;
-        if (c.slope) {
-          float p[3];
-          load_position(p, c.pos_q, query, c.axes);
-#pragma unroll
-          for (int a = 0; a < 3; ++a)
-            stage_row[a] = p[a];
-          stage_row[3] = c.slope[head] * kLog2e;
-        }
-        stage_row[4] = c.lse[(int64_t)head * c.nq + query];
-        stage_row[5] = c.delta[(int64_t)head * c.nq + query];
+  const Requests<T, DP, KT> request_q(c.q, c.d), request_do(c.dout, c.d);
+  // Two buffers: while a tile is worked on, the next one is on its way.
+  auto request = [&](int begin, int end, int buffer) {
+    char *tile = lds_tiles + buffer * 2 * TILE;
+    request_q(begin, end, group, head0, tile);
+    request_do(begin, end, group, head0, tile + TILE);
+    const int w = __builtin_amdgcn_readfirstlane(wave);
+    const int row = begin + w * 64 + lane;
+    if (w * 64 < KT && (KT >= 64 || lane < KT)) {
+      const int query = row / group, head = head0 + row - query * group;
+      auto one = [&](int what, const float *from) {
+        request4(row < end ? (const void *)from : (const void *)kZeros,
+                 lds_address(&lds_row[buffer][what][w * 64]));
+      };
+      const int64_t at = (int64_t)head * c.nq + query;
+      one(4, c.lse + at);
+      one(5, c.delta + at);
+      if (c.slope) {
+        for (int a = 0; a < c.axes; ++a)
+          one(a, c.pos_q + (int64_t)query * c.axes + a);
+        one(3, c.slope + head);
       }
     }
   };
+  if (c.axes == 2)
+    clear_lds<sizeof(lds_row)>(reinterpret_cast<char *>(lds_row));
+  if (c.d < DP)
+    clear_lds<4 * TILE>(lds_tiles);
 
   Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  int buffer = 0;
   if (walk.there())
-    fetch(walk.begin(), walk.end());
-  while (walk.there()) {
-    const int begin = walk.begin(), end = walk.end();
-    const int2 span = make_int2(spans.begin[walk.span], end);
-    __syncthreads();
-    stage_q.store(lds_q);
-    stage_do.store(lds_do);
-    if (threadIdx.x < KT) {
-#pragma unroll
-      for (int a = 0; a < 6; ++a)
-        lds_row[a][threadIdx.x] = stage_row[a];
-    }
-    __syncthreads();
+    request(walk.begin(), walk.end(), 0);
+  for (; walk.there(); buffer ^= 1) {
+    const int2 span = make_int2(walk.first(), walk.end());
+    const int begin = walk.begin(), end = span.y;
+    arrive();
     walk.next();
     if (walk.there())
-      fetch(walk.begin(), walk.end());
+      request(walk.begin(), walk.end(), buffer ^ 1);
+    const char *lds_q = lds_tiles + buffer * 2 * TILE + part * S::BYTES;
+    const char *lds_do = lds_q + TILE;
 
     bool in[RB];
     bool any = false, all = true;
@@ -1138,58 +1276,107 @@ attention_dkv_kernel(AttentionCall c) {
 
 #pragma unroll
     for (int f = 0; f < KB / S::FB; ++f) {
-      f32x4 ds[RB][S::FB], pr[RB][S::FB];
-      float top[RB];
-#pragma unroll
-      for (int rb = 0; rb < RB; ++rb)
-        top[rb] = 0.f;
+      f32x4 pr[RB][S::FB], ds[RB][S::FB], flat[RB][S::FB];
 #pragma unroll
       for (int b = 0; b < S::FB; ++b) {
-        const int kb = f * S::FB + b;
-        f32x4 s[RB], dp[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
-          s[rb] = dp[rb] = f32x4{0, 0, 0, 0};
+          pr[rb][b] = ds[rb][b] = f32x4{0, 0, 0, 0};
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
-          const u32x4 a = rows_operand<T, DP>(lds_q + part * S::PITCH, kb, ks);
-          const u32x4 b2 =
-              rows_operand<T, DP>(lds_do + part * S::PITCH, kb, ks);
+          const u32x4 aq = rows_operand<T, DP>(lds_q, f * S::FB + b, ks);
+          const u32x4 ao = rows_operand<T, DP>(lds_do, f * S::FB + b, ks);
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
-            mma<T>(s[rb], a, k[rb][ks]);
-            mma<T>(dp[rb], b2, v[rb][ks]);
-          }
-        }
-        f32x4 row[6];
-        const int at = part + kb * 16 + g * 4;
-#pragma unroll
-        for (int a = 0; a < 6; ++a)
-          row[a] = *reinterpret_cast<const f32x4 *>(&lds_row[a][at]);
-        const f32x4 pos[3] = {row[0], row[1], row[2]};
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          f32x4 flat;
-          scores<T, true>(s[rb], c, col[rb].p, pos, row[3], &flat);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float w = __builtin_amdgcn_exp2f(s[rb][r] - row[4][r]);
-            float x = w * (dp[rb][r] - row[5][r]);
-            if (c.cap > 0.f)
-              x *= flat[r];
-            if ((cut || mixed) && (!in[rb] || begin + at + r >= end))
-              w = x = 0.f;
-            pr[rb][b][r] = w * kWeightUp<T>;
-            ds[rb][b][r] = x;
-            top[rb] = fmaxf(top[rb], fabsf(x));
+            mma<T>(pr[rb][b], aq, k[rb][ks]);
+            mma<T>(ds[rb][b], ao, v[rb][ks]);
           }
         }
       }
-      if constexpr (Range<T>::on) {
-        bool moves = false;
+      cap_scores<T, true, RB, S::FB>(pr, c, flat);
+      const auto &rows = lds_row[buffer];
+      const int at = part + f * S::KF + g * 4;
+      if (c.slope) {
+#pragma unroll
+        for (int b = 0; b < S::FB; ++b) {
+          const f32x4 slope =
+              *reinterpret_cast<const f32x4 *>(&rows[3][at + b * 16]) *
+              -kLog2e;
+          const f32x4 x =
+              *reinterpret_cast<const f32x4 *>(&rows[0][at + b * 16]);
+          if (c.axes == 1) {
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                pr[rb][b][r] = fmaf(slope[r], far_by(col[rb].p, x[r]),
+                                    pr[rb][b][r]);
+          } else {
+            const f32x4 y =
+                *reinterpret_cast<const f32x4 *>(&rows[1][at + b * 16]);
+            const f32x4 z =
+                *reinterpret_cast<const f32x4 *>(&rows[2][at + b * 16]);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                pr[rb][b][r] = fmaf(slope[r],
+                                    far_by(col[rb].p, x[r], y[r], z[r]),
+                                    pr[rb][b][r]);
+          }
+        }
+      }
+#pragma unroll
+      for (int b = 0; b < S::FB; ++b) {
+        const f32x4 lse =
+            *reinterpret_cast<const f32x4 *>(&rows[4][at + b * 16]);
+        const f32x4 delta =
+            *reinterpret_cast<const f32x4 *>(&rows[5][at + b * 16]);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            pr[rb][b][r] = __builtin_amdgcn_exp2f(pr[rb][b][r] - lse[r]);
+            ds[rb][b][r] = pr[rb][b][r] * (ds[rb][b][r] - delta[r]);
+          }
+      }
+      if (c.cap > 0.f) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+            ds[rb][b] *= flat[rb][b];
+      }
+      if (cut || mixed) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (!in[rb] || begin + at + b * 16 + r >= end)
+                pr[rb][b][r] = ds[rb][b][r] = 0.f;
+      }
+      if constexpr (kWeightUp<T> != 1.f) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+            pr[rb][b] *= kWeightUp<T>;
+      }
+      if constexpr (Range<T>::on) {
+        float top[RB];
+        bool moves = false;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+          top[rb] = 0.f;
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              top[rb] = fmaxf(top[rb], fabsf(ds[rb][b][r]));
           moves |= range[rb].moves(top[rb]);
+        }
         if (__ballot(moves) != 0) {
 #pragma unroll
           for (int rb = 0; rb < RB; ++rb) {
@@ -1213,8 +1400,8 @@ attention_dkv_kernel(AttentionCall c) {
       }
 #pragma unroll
       for (int db = 0; db < S::DB; ++db) {
-        const u32x4 a = turned_operand<T, DP>(lds_do, part + f * S::KF, db);
-        const u32x4 b = turned_operand<T, DP>(lds_q, part + f * S::KF, db);
+        const u32x4 a = turned_operand<T, DP>(lds_do, f * S::KF, db);
+        const u32x4 b = turned_operand<T, DP>(lds_q, f * S::KF, db);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           if (mixed) {
@@ -1241,7 +1428,7 @@ attention_dkv_kernel(AttentionCall c) {
     for (int db = 0; db < S::DB; ++db)
       acc_k[db][rb] *= 1.f / range[rb].factor;
   if constexpr (WK > 1) {
-    static_assert(kWaves * 16 * (DP + 4) * 4 <= 2 * TILE, "sums do not fit");
+    static_assert(kWaves * 16 * (DP + 4) * 4 <= 4 * TILE, "sums do not fit");
     auto lds_acc = reinterpret_cast<float(*)[16][DP + 4]>(lds_tiles);
     join_waves<T, DP, RB, WK>(acc_k, lds_acc);
     join_waves<T, DP, RB, WK>(acc_v, lds_acc);
@@ -1260,15 +1447,12 @@ attention_dkv_kernel(AttentionCall c) {
 
 // ---- launch -------------------------------------------------------------------
 
-// Owned rows of a workgroup.
-constexpr int kWideRows = 128, kFewRows = 16;
-
 template <typename T, int DP>
 hipError_t launch(const AttentionCall &c, int pass, bool wide,
                   hipStream_t stream) {
   const int64_t owned =
       pass == 2 ? c.nk : (int64_t)c.nq * (c.hq / c.hk);
-  const int rows = wide ? kWideRows : kFewRows;
+  const int rows = wide ? wide_rows(pass, sizeof(T), DP) : kFewRows;
   const int64_t grid = (owned + rows - 1) / rows * c.hk * c.splits;
   if (grid <= 0)
     return hipSuccess;
@@ -1277,17 +1461,20 @@ hipError_t launch(const AttentionCall &c, int pass, bool wide,
   const dim3 g((unsigned)grid), b(kThreads);
   if (pass == 0) {
     if (wide)
-      attention_forward_kernel<T, DP, 2, 1><<<g, b, 0, stream>>>(c);
+      attention_forward_kernel<T, DP, wide_rows(0, sizeof(T), DP) / 64, 1>
+          <<<g, b, 0, stream>>>(c);
     else
       attention_forward_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
   } else if (pass == 1) {
     if (wide)
-      attention_dq_kernel<T, DP, 2, 1><<<g, b, 0, stream>>>(c);
+      attention_dq_kernel<T, DP, wide_rows(1, sizeof(T), DP) / 64, 1>
+          <<<g, b, 0, stream>>>(c);
     else
       attention_dq_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
   } else {
     if (wide)
-      attention_dkv_kernel<T, DP, 2, 1><<<g, b, 0, stream>>>(c);
+      attention_dkv_kernel<T, DP, wide_rows(2, sizeof(T), DP) / 64, 1>
+          <<<g, b, 0, stream>>>(c);
     else
       attention_dkv_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
   }

@@ -114,7 +114,7 @@ struct Attention {
   Tensor workspace(bool backward) const {
     const size_t bytes = pca_attention_workspace_bytes(
         q.size(0), k.size(0), (int32_t)q.size(1), (int32_t)k.size(1),
-        (int32_t)q.size(2), backward);
+        (int32_t)q.size(2), dtype_code(q), backward);
     TORCH_CHECK(bytes > 0, "attention: problem size not supported");
     return scratch(bytes, q);
   }

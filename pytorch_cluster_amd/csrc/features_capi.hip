@@ -45,8 +45,9 @@ pca::HeadRows head_rows(const void *data, int64_t row, int64_t head, int64_t d,
   r.row = row;
   r.head = head;
   const int64_t size = (int64_t)type_size(dtype);
+  // (rows of a tile, at most 128, are addressed by 32 bits)
   r.vec = on16(data) && row * size % 16 == 0 && head * size % 16 == 0 &&
-          d * size % 16 == 0;
+          d * size % 16 == 0 && row >= 0 && row * size < (1 << 24);
   return r;
 }
 
@@ -196,10 +197,12 @@ int pca_spans(const int64_t *ids_a, int64_t na, const int64_t *ids_b,
 }
 
 size_t pca_attention_workspace_bytes(int64_t nq, int64_t nk, int32_t hq,
-                                     int32_t hk, int32_t d, int backward) {
-  if (!attention_sizes_ok(nq, nk, hq, hk, d))
+                                     int32_t hk, int32_t d, int32_t dtype,
+                                     int backward) {
+  if (!attention_sizes_ok(nq, nk, hq, hk, d) || !type_ok(dtype))
     return 0;
-  return pca::attention_workspace_bytes(backward ? 1 : 0, nq, nk, hq, hk, d);
+  return pca::attention_workspace_bytes(backward ? 1 : 0, nq, nk, hq, hk, dtype,
+                                        d);
 }
 
 int pca_attention_forward(const pca_attention_args *args, void *out, float *lse,
@@ -214,7 +217,7 @@ int pca_attention_forward(const pca_attention_args *args, void *out, float *lse,
                      "attention: out has to start on 16 bytes");
   rc = no_workspace("attention",
                     pca::attention_workspace_bytes(0, c.nq, c.nk, c.hq, c.hk,
-                                                   c.d),
+                                                   args->dtype, c.d),
                     workspace, workspace_bytes);
   if (rc != PCA_OK)
     return rc;
@@ -249,7 +252,7 @@ int pca_attention_backward(const pca_attention_args *args, const void *out,
                      "attention backward: spans of one side only");
   rc = no_workspace("attention backward",
                     pca::attention_workspace_bytes(1, c.nq, c.nk, c.hq, c.hk,
-                                                   c.d),
+                                                   args->dtype, c.d),
                     workspace, workspace_bytes);
   if (rc != PCA_OK)
     return rc;

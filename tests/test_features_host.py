@@ -147,8 +147,9 @@ def test_c_abi_checks_before_any_launch():
     assert forward(size=16) == -3
     assert forward(ws=at + 8) == -3
     assert forward(ws=None) == -3
-    assert lib.pca_attention_workspace_bytes(10, 10, 4, 3, 64, 0) == 0
-    assert lib.pca_attention_workspace_bytes(10, 10, 4, 2, 64, 1) > 0
+    assert lib.pca_attention_workspace_bytes(10, 10, 4, 3, 64, 0, 0) == 0
+    assert lib.pca_attention_workspace_bytes(10, 10, 4, 2, 64, 0, 1) > 0
+    assert lib.pca_attention_workspace_bytes(10, 10, 4, 2, 64, 1, 1) == 0
 
     def backward(dq=at, lse=at, **change):
         a = _native.AttentionArgs.from_buffer_copy(args)
