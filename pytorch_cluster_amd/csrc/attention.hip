@@ -11,22 +11,25 @@ namespace {
 
 size_t attn_align(size_t v) { return (v + 255) & ~(size_t)255; }
 
-// First entry of the sorted `ids` at [lo, hi) that is not below `id` (`above`: that is
-// above it).
-__device__ __forceinline__ int bound_of(const int64_t *ids, int lo, int hi,
-                                        int64_t id, bool above) {
-  while (lo < hi) {
-    const int mid = lo + ((hi - lo) >> 1);
-    const int64_t v = ids[mid];
-    if (v < id || (above && v == id))
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  return lo;
+// One step of a search in the sorted `ids`: [lo, hi] holds the first entry that is not
+// below `id` (`above`: that is above it); eight places are looked at at once.
+__device__ __forceinline__ void search_step(const int64_t *ids, int &lo, int &hi,
+                                            int64_t id, bool above) {
+  const int n = hi - lo, step = n / 8 + 1;
+  int64_t v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    v[k] = ids[min(lo + k * step, hi - 1)];
+  int below = 0;
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    below += lo + k * step < hi && (v[k] < id || (above && v[k] == id));
+  hi = below == 0 ? lo : min(lo + below * step, hi);
+  lo = below == 0 ? lo : lo + (below - 1) * step + 1;
 }
 
-// The same by the lanes of a wave, 64 places at a time.
+// First entry of the sorted `ids` that is not below `id` (`above`: that is above it), by
+// the lanes of a wave, 64 places at a time.
 __device__ __forceinline__ int wave_bound_of(const int64_t *ids, int n,
                                              int64_t id, bool above) {
   const int lane = threadIdx.x & 63;
@@ -81,8 +84,15 @@ __global__ __launch_bounds__(256) void spans_kernel(const int64_t *ids_a, int na
   int2 v = make_int2(lo, hi);
   if (id_first != id_last) {
     const int64_t id = ids_a[i];
-    v.x = bound_of(ids_b, lo, hi, id, false);
-    v.y = bound_of(ids_b, v.x, hi, id, true);
+    int lo_end = lo, hi_end = hi, hi_begin = hi;
+    v.x = lo;
+    while (v.x < hi_begin || lo_end < hi_end) {
+      if (v.x < hi_begin)
+        search_step(ids_b, v.x, hi_begin, id, false);
+      if (lo_end < hi_end)
+        search_step(ids_b, lo_end, hi_end, id, true);
+    }
+    v.y = max(v.x, lo_end);
   }
   spans[i] = v;
 }
@@ -101,31 +111,73 @@ __device__ __forceinline__ void put_as(int dtype, void *out, int64_t at,
     put<__bf16>(out, at, v);
 }
 
-// Output rows from the pieces' sums, maxima and sums of weights: 32 lanes a row, four
-// elements each.
-__global__ __launch_bounds__(256) void join_forward_kernel(AttentionCall c,
-                                                           int dtype) {
+// Output rows from the pieces' sums, maxima and sums of weights: 32 lanes take four
+// elements each; where there are many pieces, `shares` groups of lanes divide them and
+// meet in LDS, in their order.
+__global__ __launch_bounds__(256) void
+join_forward_kernel(AttentionCall c, int dtype, int shares) {
+  __shared__ float lds_acc[8][128], lds_ml[8][2];
   const int64_t rows = (int64_t)c.nq * c.hq;
-  const int64_t row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  if (row >= rows)
-    return;
-  float top = -__builtin_inff(), sum = 0.f;
-  for (int s = 0; s < c.splits; ++s)
-    top = fmaxf(top, c.part_ml[(s * rows + row) * 2]);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const int grp = threadIdx.x / 32, share = grp % shares;
+  const int64_t row = (int64_t)blockIdx.x * (8 / shares) + grp / shares;
+  const bool there = row < rows;
   const int e0 = (threadIdx.x & 31) * 4;
-  for (int s = 0; s < c.splits; ++s) {
-    const float m = c.part_ml[(s * rows + row) * 2];
-    const float l = c.part_ml[(s * rows + row) * 2 + 1];
-    if (m == -__builtin_inff() && l == 0.f)
-      continue; // nothing in this piece
-    const float w = m == top ? 1.f : __builtin_amdgcn_exp2f(m - top);
-    sum += l * w;
+  float top = -__builtin_inff(), sum = 0.f;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (there) {
+    for (int s = share; s < c.splits; s += shares)
+      top = fmaxf(top, c.part_ml[(s * rows + row) * 2]);
+#pragma unroll 4
+    for (int s = share; s < c.splits; s += shares) {
+      const float m = c.part_ml[(s * rows + row) * 2];
+      const float l = c.part_ml[(s * rows + row) * 2 + 1];
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+      const float *from = c.part + (s * rows + row) * c.d + e0;
+      if (c.d % 4 == 0) {
+        if (e0 < c.d)
+          __builtin_memcpy(v, __builtin_assume_aligned(from, 16), 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = e0 + e < c.d ? from[e] : 0.f;
+      }
+      // (-inf: nothing in this piece)
+      const float w = m == -__builtin_inff() ? 0.f
+                      : m == top             ? 1.f
+                                 : __builtin_amdgcn_exp2f(m - top);
+      sum = fmaf(l, w, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[e] = fmaf(v[e], w, acc[e]);
+    }
+  }
+  if (shares > 1) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (e0 + e < c.d)
-        acc[e] = fmaf(c.part[(s * rows + row) * c.d + e0 + e], w, acc[e]);
+      lds_acc[grp][e0 + e] = acc[e];
+    if (e0 == 0) {
+      lds_ml[grp][0] = top;
+      lds_ml[grp][1] = sum;
+    }
+    __syncthreads();
+    if (share != 0)
+      return;
+    for (int k = 1; k < shares; ++k)
+      top = fmaxf(top, lds_ml[grp + k][0]);
+    sum = acc[0] = acc[1] = acc[2] = acc[3] = 0.f;
+    for (int k = 0; k < shares; ++k) {
+      const float m = lds_ml[grp + k][0];
+      const float w = m == -__builtin_inff() ? 0.f
+                      : m == top             ? 1.f
+                                 : __builtin_amdgcn_exp2f(m - top);
+      sum = fmaf(lds_ml[grp + k][1], w, sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        acc[e] = fmaf(lds_acc[grp + k][e0 + e], w, acc[e]);
+    }
   }
+  if (!there)
+    return;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
@@ -179,17 +231,17 @@ AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
   const int64_t rows_q = nq * (hq / hk);
   const int64_t owned = pass == 2 ? nk : rows_q;
   const int64_t looped = pass == 2 ? rows_q : nk;
+  auto groups = [&](int rows) { return (owned + rows - 1) / rows * hk; };
   AttentionPlan p;
-  const int rows = wide_rows(pass, dtype == 0 ? 4 : 2, d);
-  const int64_t wide = (owned + rows - 1) / rows * hk;
-  p.wide = wide >= 256;
-  if (!p.wide) {
-    const int64_t few =
-        std::max<int64_t>(1, (owned + kFewRows - 1) / kFewRows * hk);
-    const int64_t most = (looped + 255) / 256;
-    p.splits = (int)std::clamp<int64_t>(1024 / few, 1,
-                                        std::clamp<int64_t>(most, 1, 256));
-  }
+  p.rows = most_rows(pass, dtype == 0 ? 4 : 2, d);
+  if (d <= 32 || (d <= 64 && pass != 2) || groups(p.rows) < 512)
+    p.rows = 64;
+  if (owned <= 256)
+    p.rows = kFewRows;
+  const int64_t n = std::max<int64_t>(1, groups(p.rows));
+  const int64_t want = p.rows == kFewRows ? 512 : n < 800 ? 2048 : 0;
+  p.splits = (int)std::clamp<int64_t>(
+      (want + n / 2) / n, 1, std::clamp<int64_t>(looped / 128, 1, 64));
   return p;
 }
 
@@ -222,12 +274,14 @@ hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
   c.part_ml = c.part + attn_align(sizeof(float) * (size_t)p.splits * c.nq *
                                   c.hq * c.d) /
                            sizeof(float);
-  hipError_t e = launcher(dtype, c.d)(c, 0, p.wide, stream);
+  hipError_t e = launcher(dtype, c.d)(c, 0, p.rows, stream);
   if (e != hipSuccess || p.splits == 1 || c.nq == 0)
     return e;
-  const int64_t blocks = ((int64_t)c.nq * c.hq + 7) / 8;
-  join_forward_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(c,
-                                                                        dtype);
+  const int shares = p.splits >= 32 ? 8 : p.splits >= 16 ? 4 : 1;
+  const int64_t blocks =
+      ((int64_t)c.nq * c.hq + 8 / shares - 1) / (8 / shares);
+  join_forward_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
+      c, dtype, shares);
   return hipGetLastError();
 }
 
@@ -238,7 +292,7 @@ hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
            attn_align(sizeof(float) * (size_t)c.nq * c.hq) / sizeof(float);
   const AttentionPlan pq = attention_plan(1, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
   c.splits = pq.splits;
-  hipError_t e = launcher(dtype, c.d)(c, 1, pq.wide, stream);
+  hipError_t e = launcher(dtype, c.d)(c, 1, pq.rows, stream);
   if (e == hipSuccess && c.splits > 1 && c.nq > 0) {
     const int64_t count = (int64_t)c.nq * c.hq * c.d;
     e = join_sum(c, c.part, count, count, dtype, c.dq, stream);
@@ -247,7 +301,7 @@ hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
     return e;
   const AttentionPlan pk = attention_plan(2, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
   c.splits = pk.splits;
-  e = launcher(dtype, c.d)(c, 2, pk.wide, stream);
+  e = launcher(dtype, c.d)(c, 2, pk.rows, stream);
   if (e == hipSuccess && c.splits > 1 && c.nk > 0) {
     const int64_t count = (int64_t)c.nk * c.hk * c.d;
     e = join_sum(c, c.part, 2 * count, count, dtype, c.dk, stream);

@@ -43,33 +43,34 @@ struct AttentionCall {
   float *part_ml = nullptr; // forward: [splits, nq, hq, 2]
 };
 
-// Which of the kernels of a pass runs, and in how many pieces.
+// Which of the kernels of a pass runs (owned rows of a workgroup), and in how many
+// pieces.
 struct AttentionPlan {
-  bool wide = true;
+  int rows = 128;
   int splits = 1;
 };
 
 // One per element type (0 fp32, 2 fp16, 3 bf16: pca_dtype) and width of a head (32,
 // 64, 128): attention_<type>_d<width>.hip.  `pass`: 0 forward, 1 dq, 2 dk and dv.
 typedef hipError_t (*AttentionLauncher)(const AttentionCall &, int pass,
-                                        bool wide, hipStream_t);
+                                        int rows, hipStream_t);
 #define PCA_ATTENTION_DECLARE(type)                                            \
-  hipError_t attention_##type##_d32(const AttentionCall &, int, bool,          \
+  hipError_t attention_##type##_d32(const AttentionCall &, int, int,           \
                                     hipStream_t);                              \
-  hipError_t attention_##type##_d64(const AttentionCall &, int, bool,          \
+  hipError_t attention_##type##_d64(const AttentionCall &, int, int,           \
                                     hipStream_t);                              \
-  hipError_t attention_##type##_d128(const AttentionCall &, int, bool,         \
+  hipError_t attention_##type##_d128(const AttentionCall &, int, int,          \
                                      hipStream_t)
 PCA_ATTENTION_DECLARE(f32);
 PCA_ATTENTION_DECLARE(f16);
 PCA_ATTENTION_DECLARE(bf16);
 #undef PCA_ATTENTION_DECLARE
 
-// Owned rows of a workgroup: of the kernels whose waves own rows of their own, and of
-// those for few rows.  Two blocks of 16 columns per wave share every left operand; where
-// the sums of both do not fit the registers of two waves per SIMD it is one.
+// Owned rows of a workgroup: 16 (its waves divide the looped rows), 64 or at most this
+// many.  Two blocks of 16 columns per wave share every left operand; where the sums of
+// both do not fit the registers of two waves per SIMD it is one.
 constexpr int kFewRows = 16;
-constexpr int wide_rows(int pass, int size, int width) {
+constexpr int most_rows(int pass, int size, int width) {
   return width > 64 && (pass == 2 || (pass == 1 && size == 4)) ? 64 : 128;
 }
 

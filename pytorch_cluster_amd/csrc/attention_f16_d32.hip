@@ -2,8 +2,8 @@
 #include "attention_impl.hpp"
 
 namespace pca {
-hipError_t attention_f16_d32(const AttentionCall &c, int pass, bool wide,
-                  hipStream_t stream) {
-  return attn::launch<_Float16, 32>(c, pass, wide, stream);
+hipError_t attention_f16_d32(const AttentionCall &c, int pass, int rows,
+                          hipStream_t stream) {
+  return attn::launch<_Float16, 32>(c, pass, rows, stream);
 }
 } // namespace pca

@@ -165,14 +165,18 @@ template <typename T, int DP, int ROWS> struct Requests {
   const HeadRows &x;
   int d, wave;
   uint32_t offset[LANES]; // bytes of this thread's first pieces from a tile's row
+  bool on[LANES];         // they lie in d
 
   __device__ __forceinline__ Requests(const HeadRows &rows, int width)
       : x(rows), d(width) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int l = 0; l < LANES; ++l)
-      offset[l] = (uint32_t)((threadIdx.x / S::CH) * x.row * S::SZ) +
-                  piece(threadIdx.x / S::CH + l * STEP) * 16;
+    for (int l = 0; l < LANES; ++l) {
+      const int p = piece(threadIdx.x / S::CH + l * STEP);
+      offset[l] =
+          (uint32_t)((threadIdx.x / S::CH) * x.row * S::SZ) + p * 16;
+      on[l] = p * S::PER < d;
+    }
   }
   __device__ __forceinline__ static int piece(int row) {
     return threadIdx.x % S::CH ^ S::turn(row);
@@ -184,11 +188,14 @@ template <typename T, int DP, int ROWS> struct Requests {
       const char *base = static_cast<const char *>(x.data) +
                          ((int64_t)begin * x.row + (int64_t)head0 * x.head) *
                              S::SZ;
+      const int64_t step = (int64_t)STEP * x.row * S::SZ;
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (piece(threadIdx.x / S::CH + e * STEP) * S::PER < d)
-          request16(base + (int64_t)(e * STEP) * x.row * S::SZ,
-                    offset[e % LANES], lds + kWaves * e * 1024);
+      for (int l = 0; l < LANES; ++l)
+        if (on[l]) {
+#pragma unroll
+          for (int e = l; e < N; e += LANES)
+            request16(base + e * step, offset[l], lds + kWaves * e * 1024);
+        }
       return;
     }
 #pragma unroll 1
@@ -311,23 +318,19 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
-// tanh(x / 2 log2 e)... of a score: t = tanh of `x` times log 2 / 2, that is
-// (exp2(x) - 1) / (exp2(x) + 1).  Near 0 the difference would lose what fp32 rows
-// need, so there the series is used: x log 2 / 2 below 0.35 (error 2e-8 relative).
-template <typename T> __device__ __forceinline__ float tanh_of(float x) {
+// tanh y for fp32 rows, x = 2 y log2 e: (exp2(x) - 1) / (exp2(x) + 1), and near 0,
+// where that difference would lose digits, the series (error 2e-8 relative below 0.35).
+__device__ __forceinline__ float tanh_of(float x) {
   const float e = __builtin_amdgcn_exp2f(x);
   const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
-  if constexpr (std::is_same<T, float>::value) {
-    const float y = x * 0.34657359027997264f, z = y * y;
-    const float near =
-        y + y * z *
-                (-0.33333333333f +
-                 z * (0.13333333333f +
-                      z * (-0.05396825397f +
-                           z * (0.02186948854f + z * -0.00886323553f))));
-    return fabsf(y) < 0.35f ? near : far;
-  }
-  return far;
+  const float y = x * 0.34657359027997264f, z = y * y;
+  const float near =
+      y + y * z *
+              (-0.33333333333f +
+               z * (0.13333333333f +
+                    z * (-0.05396825397f +
+                         z * (0.02186948854f + z * -0.00886323553f))));
+  return fabsf(y) < 0.35f ? near : far;
 }
 
 // Spans of the rows that a workgroup owns, in order, each cut into tiles.
@@ -398,38 +401,38 @@ collect_spans(Spans<ROWS> &s, const int2 *spans, int row0, int rows, int group,
   __syncthreads();
 }
 
-// The tiles of this workgroup's piece, in order.
+// The tiles of this workgroup's piece, in order: rows [begin, end of the tile or of its
+// span).  All of it is the same in every lane and kept in scalar registers.
 template <int ROWS> struct Walk {
   const Spans<ROWS> &s;
-  int at, stop, span, tile;
+  int left, span, first, begin, end, tile;
   __device__ __forceinline__ Walk(const Spans<ROWS> &spans, int piece,
                                   int pieces, int tile_rows)
-      : s(spans), tile(tile_rows) {
-    const int total = s.count > 0 ? s.first[s.count] : 0;
-    at = (int)((int64_t)total * piece / pieces);
-    stop = (int)((int64_t)total * (piece + 1) / pieces);
-    span = 0;
-    settle();
-  }
-  __device__ __forceinline__ void settle() {
-    if (at < stop)
-      while (s.first[span + 1] <= at)
+      : s(spans), span(0), first(0), begin(0), end(0), tile(tile_rows) {
+    const int count = __builtin_amdgcn_readfirstlane(s.count);
+    const int total =
+        count > 0 ? __builtin_amdgcn_readfirstlane(s.first[count]) : 0;
+    const int at = (int)((int64_t)total * piece / pieces);
+    left = (int)((int64_t)total * (piece + 1) / pieces) - at;
+    if (left > 0) {
+      while (__builtin_amdgcn_readfirstlane(s.first[span + 1]) <= at)
         ++span;
+      enter();
+      begin += (at - __builtin_amdgcn_readfirstlane(s.first[span])) * tile;
+    }
   }
-  __device__ __forceinline__ bool there() const { return at < stop; }
-  __device__ __forceinline__ int first() const {
-    return __builtin_amdgcn_readfirstlane(s.begin[span]);
+  __device__ __forceinline__ void enter() {
+    first = begin = __builtin_amdgcn_readfirstlane(s.begin[span]);
+    end = __builtin_amdgcn_readfirstlane(s.end[span]);
   }
-  __device__ __forceinline__ int begin() const {
-    return __builtin_amdgcn_readfirstlane(s.begin[span] +
-                                          (at - s.first[span]) * tile);
-  }
-  __device__ __forceinline__ int end() const {
-    return __builtin_amdgcn_readfirstlane(s.end[span]);
-  }
+  __device__ __forceinline__ bool there() const { return left > 0; }
   __device__ __forceinline__ void next() {
-    ++at;
-    settle();
+    --left;
+    begin += tile;
+    if (begin >= end && left > 0) { // (no span is empty)
+      ++span;
+      enter();
+    }
   }
 };
 
@@ -488,34 +491,55 @@ __device__ __forceinline__ Column query_column(const AttentionCall &c, int row,
   return r;
 }
 
-// Scores in units of log 2, from the products of RB x NB blocks.  Leaves 1 - tanh^2 in
-// `flat` if asked for.
-template <typename T, bool FLAT, int RB, int NB>
-__device__ __forceinline__ void cap_scores(f32x4 (&s)[RB][NB],
-                                           const AttentionCall &c,
-                                           f32x4 (*flat)[NB]) {
-  if (c.cap > 0.f) {
-    const float in = c.scale / c.cap * (2.f * kLog2e), out = c.cap * kLog2e;
+// Which of a wave's columns a span belongs to.
+template <int RB> struct Members {
+  int span = -1;
+  bool in[RB];
+  bool some = false, mixed = false; // any column; some and not all
+  __device__ __forceinline__ void of(int number, int begin, int end,
+                                     const Column (&col)[RB]) {
+    if (number == span)
+      return;
+    span = number;
+    bool any = false, all = true;
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
+    for (int rb = 0; rb < RB; ++rb) {
+      in[rb] = col[rb].span.x == begin && col[rb].span.y == end;
+      any |= in[rb] && col[rb].valid;
+      all &= in[rb] || !col[rb].valid;
+    }
+    some = __ballot(any) != 0;
+    mixed = __ballot(!all) != 0;
+  }
+};
+
+// Scores in units of log 2 less `base` (per block and row of it), from products.  With
+// a cap, `flat` gets 1 - tanh^2 (in fp32) or a quarter of it: kFlatUp.
+template <typename T>
+constexpr float kFlatUp = std::is_same<T, float>::value ? 1.f : 4.f;
+
+template <typename T, bool FLAT>
+__device__ __forceinline__ void cap_scores(f32x4 &s, const AttentionCall &c,
+                                           f32x4 base, f32x4 *flat) {
+  const float in = c.scale / c.cap * (2.f * kLog2e), out = c.cap * kLog2e;
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float t = tanh_of<T>(s[rb][b][r] * in);
-          s[rb][b][r] = t * out;
-          if constexpr (FLAT)
-            flat[rb][b][r] = fmaf(-t, t, 1.f);
-        }
-  } else {
-    const float in = c.scale * kLog2e;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb)
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-        s[rb][b] *= in;
+  for (int r = 0; r < 4; ++r) {
+    if constexpr (std::is_same<T, float>::value) {
+      const float t = tanh_of(s[r] * in);
+      s[r] = fmaf(t, out, -base[r]);
+      if constexpr (FLAT)
+        (*flat)[r] = fmaf(-t, t, 1.f);
+    } else {
+      // tanh = 1 - 2 w, 1 - tanh^2 = 4 (w - w^2)
+      const float w =
+          __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * in) + 1.f);
+      s[r] = fmaf(w, -2.f * out, out - base[r]);
+      if constexpr (FLAT)
+        (*flat)[r] = fmaf(-w, w, w);
+    }
   }
 }
+__device__ __forceinline__ f32x4 all4(float v) { return f32x4{v, v, v, v}; }
 
 // Takes slope times distance off: p of the columns, `pos` of the looped rows.
 __device__ __forceinline__ float far_by(const float (&p)[3], float x) {
@@ -603,14 +627,17 @@ attention_forward_kernel(AttentionCall c) {
   const Place place((rows + ROWS - 1) / ROWS, c.hk, c.splits);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
-  const int wq = wave / WK, part = wave % WK * KW;
+  const int wq = wave / WK;
+  const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS;
-  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
 
   Column col[RB];
   u32x4 q[RB][S::KS];
   f32x4 acc[S::DB][RB];
+  // what is subtracted from the scores, the weights' sum (of this lane's rows), and
+  // whether there has been a row
   float m[RB], l[RB];
+  bool seen[RB];
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb) {
     col[rb] = query_column(c, row0 + (wq * RB + rb) * 16 + i, group,
@@ -625,11 +652,12 @@ attention_forward_kernel(AttentionCall c) {
 #pragma unroll
     for (int db = 0; db < S::DB; ++db)
       acc[db][rb] = f32x4{0, 0, 0, 0};
-    m[rb] = -__builtin_inff();
-    l[rb] = 0.f;
+    m[rb] = l[rb] = 0.f;
+    seen[rb] = false;
   }
 
   const Requests<T, DP, KT> request_k(c.k, c.d), request_v(c.v, c.d);
+  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
   // Two buffers: while a tile is worked on, the next one is on its way.
   auto request = [&](int begin, int end, int buffer) {
     char *tile = lds_tiles + buffer * 2 * TILE;
@@ -645,29 +673,23 @@ attention_forward_kernel(AttentionCall c) {
 
   Walk<ROWS> walk(spans, place.piece, c.splits, KT);
   int buffer = 0;
+  Members<RB> members;
   if (walk.there())
-    request(walk.begin(), walk.end(), 0);
+    request(walk.begin, walk.end, 0);
   for (; walk.there(); buffer ^= 1) {
-    const int2 span = make_int2(walk.first(), walk.end());
-    const int begin = walk.begin(), end = span.y;
+    const int begin = walk.begin, end = walk.end;
+    members.of(walk.span, walk.first, end, col);
     arrive();
     walk.next();
     if (walk.there())
-      request(walk.begin(), walk.end(), buffer ^ 1);
+      request(walk.begin, walk.end, buffer ^ 1);
     const char *lds_k = lds_tiles + buffer * 2 * TILE + part * S::BYTES;
     const char *lds_v = lds_k + TILE;
 
-    bool in[RB];
-    bool any = false, all = true;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      in[rb] = col[rb].span.x == span.x && col[rb].span.y == span.y;
-      any |= in[rb] && col[rb].valid;
-      all &= in[rb] || !col[rb].valid;
-    }
-    if (__ballot(any) == 0 || begin + part >= end)
+    if (!members.some || begin + part >= end)
       continue;
-    const bool mixed = __ballot(!all) != 0;
+    const bool(&in)[RB] = members.in;
+    const bool mixed = members.mixed;
     const bool cut = begin + part + KW > end;
 
     f32x4 s[RB][KB];
@@ -686,7 +708,22 @@ attention_forward_kernel(AttentionCall c) {
           mma<T>(s[rb][kb], a, q[rb][ks]);
       }
 
-    cap_scores<T, false, RB, KB>(s, c, nullptr);
+    if (c.cap > 0.f) {
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+          cap_scores<T, false>(s[rb][kb], c, all4(m[rb]), nullptr);
+    } else {
+      const float in = c.scale * kLog2e;
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[rb][kb][r] = fmaf(s[rb][kb][r], in, -m[rb]);
+    }
     if (c.slope)
       take_distance<RB, KB>(s, c, col, lds_pos[buffer], part);
     if (cut || mixed) {
@@ -710,40 +747,44 @@ attention_forward_kernel(AttentionCall c) {
           top[rb] = fmaxf(top[rb], s[rb][kb][r]);
     }
 
-    // The maximum that is subtracted moves only when it would grow by more than 8
-    // (256-fold sums, far from any limit): most tiles leave the sums as they are.
-    bool grow = false;
+    // What is subtracted moves only when a score would be above it by more than 8
+    // (256-fold weights, far from any limit): most tiles leave the sums as they are.
+    bool move[RB], moves = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       top[rb] = across_groups_max(top[rb]);
-      grow |= top[rb] > m[rb] + 8.f;
+      move[rb] = top[rb] > 8.f || (!seen[rb] && top[rb] > -__builtin_inff());
+      moves |= move[rb];
     }
-    if (__ballot(grow) != 0) {
+    if (__ballot(moves) != 0) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const float now = fmaxf(m[rb], top[rb]);
-        const float keep = now == -__builtin_inff()
-                               ? 1.f
-                               : __builtin_amdgcn_exp2f(m[rb] - now);
-        m[rb] = now;
+        const float by = move[rb] ? top[rb] : 0.f;
+        const float keep =
+            move[rb] && seen[rb] ? __builtin_amdgcn_exp2f(-by) : 1.f;
+        seen[rb] |= move[rb];
+        m[rb] += by;
         l[rb] *= keep;
 #pragma unroll
         for (int db = 0; db < S::DB; ++db)
           acc[db][rb] *= keep;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            s[rb][kb][r] -= by;
       }
     }
 #pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      const float base = m[rb] == -__builtin_inff() ? 0.f : m[rb];
+    for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float e = __builtin_amdgcn_exp2f(s[rb][kb][r] - base);
+          const float e = __builtin_amdgcn_exp2f(s[rb][kb][r]);
           s[rb][kb][r] = e;
           l[rb] += e;
         }
-    }
 
 #pragma unroll
     for (int f = 0; f < KB / S::FB; ++f) {
@@ -770,6 +811,10 @@ attention_forward_kernel(AttentionCall c) {
     }
   }
 
+#pragma unroll
+  for (int rb = 0; rb < RB; ++rb)
+    if (!seen[rb])
+      m[rb] = -__builtin_inff(); // nothing to be put together with others
 #pragma unroll
   for (int rb = 0; rb < RB; ++rb)
     l[rb] = across_groups_sum(l[rb]);
@@ -954,9 +999,9 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
   const Place place((rows + ROWS - 1) / ROWS, c.hk, c.splits);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
-  const int wq = wave / WK, part = wave % WK * KW;
+  const int wq = wave / WK;
+  const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS;
-  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
 
   Column col[RB];
   u32x4 q[RB][S::KS], dout[RB][S::KS];
@@ -1006,6 +1051,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
   }
 
   const Requests<T, DP, KT> request_k(c.k, c.d), request_v(c.v, c.d);
+  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
   // Two buffers: while a tile is worked on, the next one is on its way.
   auto request = [&](int begin, int end, int buffer) {
     char *tile = lds_tiles + buffer * 2 * TILE;
@@ -1021,29 +1067,23 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
 
   Walk<ROWS> walk(spans, place.piece, c.splits, KT);
   int buffer = 0;
+  Members<RB> members;
   if (walk.there())
-    request(walk.begin(), walk.end(), 0);
+    request(walk.begin, walk.end, 0);
   for (; walk.there(); buffer ^= 1) {
-    const int2 span = make_int2(walk.first(), walk.end());
-    const int begin = walk.begin(), end = span.y;
+    const int begin = walk.begin, end = walk.end;
+    members.of(walk.span, walk.first, end, col);
     arrive();
     walk.next();
     if (walk.there())
-      request(walk.begin(), walk.end(), buffer ^ 1);
+      request(walk.begin, walk.end, buffer ^ 1);
     const char *lds_k = lds_tiles + buffer * 2 * TILE + part * S::BYTES;
     const char *lds_v = lds_k + TILE;
 
-    bool in[RB];
-    bool any = false, all = true;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      in[rb] = col[rb].span.x == span.x && col[rb].span.y == span.y;
-      any |= in[rb] && col[rb].valid;
-      all &= in[rb] || !col[rb].valid;
-    }
-    if (__ballot(any) == 0 || begin + part >= end)
+    if (!members.some || begin + part >= end)
       continue;
-    const bool mixed = __ballot(!all) != 0;
+    const bool(&in)[RB] = members.in;
+    const bool mixed = members.mixed;
     const bool cut = begin + part + KW > end;
 
 #pragma unroll
@@ -1053,7 +1093,10 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
       for (int b = 0; b < S::FB; ++b) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
-          s[rb][b] = ds[rb][b] = f32x4{0, 0, 0, 0};
+          s[rb][b] = f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+          ds[rb][b] = all4(-delta[rb]);
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
           const u32x4 ak = rows_operand<T, DP>(lds_k, f * S::FB + b, ks);
@@ -1065,7 +1108,22 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
           }
         }
       }
-      cap_scores<T, true, RB, S::FB>(s, c, flat);
+      if (c.cap > 0.f) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+            cap_scores<T, true>(s[rb][b], c, all4(lse[rb]), &flat[rb][b]);
+      } else {
+        const float in = c.scale * kLog2e;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              s[rb][b][r] = fmaf(s[rb][b][r], in, -lse[rb]);
+      }
       if (c.slope)
         take_distance<RB, S::FB>(s, c, col, lds_pos[buffer], part + f * S::KF);
 #pragma unroll
@@ -1074,8 +1132,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
         for (int b = 0; b < S::FB; ++b)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            ds[rb][b][r] = __builtin_amdgcn_exp2f(s[rb][b][r] - lse[rb]) *
-                           (ds[rb][b][r] - delta[rb]);
+            ds[rb][b][r] *= __builtin_amdgcn_exp2f(s[rb][b][r]);
       if (c.cap > 0.f) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
@@ -1163,7 +1220,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
           c.splits > 1
               ? c.part + (int64_t)place.piece * c.nq * c.hq * c.d
               : nullptr;
-      store_columns<T, DP, RB, WK>(acc, rb, c.dq, piece, at, c.d, c.scale);
+      store_columns<T, DP, RB, WK>(acc, rb, c.dq, piece, at, c.d,
+                                   c.cap > 0.f ? c.scale * kFlatUp<T> : c.scale);
     }
 }
 
@@ -1185,9 +1243,9 @@ attention_dkv_kernel(AttentionCall c) {
   const Place place((c.nk + ROWS - 1) / ROWS, c.hk, c.splits);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
-  const int wq = wave / WK, part = wave % WK * KW;
+  const int wq = wave / WK;
+  const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS, head0 = place.head * group;
-  collect_spans<ROWS>(spans, c.spans_k, row0, c.nk, 1, c.nq, group, KT);
 
   Column col[RB];
   u32x4 k[RB][S::KS], v[RB][S::KS];
@@ -1219,6 +1277,7 @@ attention_dkv_kernel(AttentionCall c) {
   }
 
   const Requests<T, DP, KT> request_q(c.q, c.d), request_do(c.dout, c.d);
+  collect_spans<ROWS>(spans, c.spans_k, row0, c.nk, 1, c.nq, group, KT);
   // Two buffers: while a tile is worked on, the next one is on its way.
   auto request = [&](int begin, int end, int buffer) {
     char *tile = lds_tiles + buffer * 2 * TILE;
@@ -1249,39 +1308,40 @@ attention_dkv_kernel(AttentionCall c) {
 
   Walk<ROWS> walk(spans, place.piece, c.splits, KT);
   int buffer = 0;
+  Members<RB> members;
   if (walk.there())
-    request(walk.begin(), walk.end(), 0);
+    request(walk.begin, walk.end, 0);
   for (; walk.there(); buffer ^= 1) {
-    const int2 span = make_int2(walk.first(), walk.end());
-    const int begin = walk.begin(), end = span.y;
+    const int begin = walk.begin, end = walk.end;
+    members.of(walk.span, walk.first, end, col);
     arrive();
     walk.next();
     if (walk.there())
-      request(walk.begin(), walk.end(), buffer ^ 1);
+      request(walk.begin, walk.end, buffer ^ 1);
     const char *lds_q = lds_tiles + buffer * 2 * TILE + part * S::BYTES;
     const char *lds_do = lds_q + TILE;
 
-    bool in[RB];
-    bool any = false, all = true;
-#pragma unroll
-    for (int rb = 0; rb < RB; ++rb) {
-      in[rb] = col[rb].span.x == span.x && col[rb].span.y == span.y;
-      any |= in[rb] && col[rb].valid;
-      all &= in[rb] || !col[rb].valid;
-    }
-    if (__ballot(any) == 0 || begin + part >= end)
+    if (!members.some || begin + part >= end)
       continue;
-    const bool mixed = __ballot(!all) != 0;
+    const bool(&in)[RB] = members.in;
+    const bool mixed = members.mixed;
     const bool cut = begin + part + KW > end;
 
 #pragma unroll
     for (int f = 0; f < KB / S::FB; ++f) {
-      f32x4 pr[RB][S::FB], ds[RB][S::FB], flat[RB][S::FB];
+      f32x4 pr[RB][S::FB], ds[RB][S::FB], flat[RB][S::FB], lse[S::FB];
+      const auto &rows = lds_row[buffer];
+      const int at = part + f * S::KF + g * 4;
 #pragma unroll
       for (int b = 0; b < S::FB; ++b) {
+        lse[b] = *reinterpret_cast<const f32x4 *>(&rows[4][at + b * 16]);
+        const f32x4 delta =
+            *reinterpret_cast<const f32x4 *>(&rows[5][at + b * 16]);
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb)
-          pr[rb][b] = ds[rb][b] = f32x4{0, 0, 0, 0};
+        for (int rb = 0; rb < RB; ++rb) {
+          pr[rb][b] = f32x4{0, 0, 0, 0};
+          ds[rb][b] = -delta;
+        }
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
           const u32x4 aq = rows_operand<T, DP>(lds_q, f * S::FB + b, ks);
@@ -1293,9 +1353,22 @@ attention_dkv_kernel(AttentionCall c) {
           }
         }
       }
-      cap_scores<T, true, RB, S::FB>(pr, c, flat);
-      const auto &rows = lds_row[buffer];
-      const int at = part + f * S::KF + g * 4;
+      if (c.cap > 0.f) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+            cap_scores<T, true>(pr[rb][b], c, lse[b], &flat[rb][b]);
+      } else {
+        const float in = c.scale * kLog2e;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+          for (int b = 0; b < S::FB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              pr[rb][b][r] = fmaf(pr[rb][b][r], in, -lse[b][r]);
+      }
       if (c.slope) {
 #pragma unroll
         for (int b = 0; b < S::FB; ++b) {
@@ -1327,19 +1400,14 @@ attention_dkv_kernel(AttentionCall c) {
         }
       }
 #pragma unroll
-      for (int b = 0; b < S::FB; ++b) {
-        const f32x4 lse =
-            *reinterpret_cast<const f32x4 *>(&rows[4][at + b * 16]);
-        const f32x4 delta =
-            *reinterpret_cast<const f32x4 *>(&rows[5][at + b * 16]);
+      for (int b = 0; b < S::FB; ++b)
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            pr[rb][b][r] = __builtin_amdgcn_exp2f(pr[rb][b][r] - lse[r]);
-            ds[rb][b][r] = pr[rb][b][r] * (ds[rb][b][r] - delta[r]);
+            pr[rb][b][r] = __builtin_amdgcn_exp2f(pr[rb][b][r]);
+            ds[rb][b][r] *= pr[rb][b][r];
           }
-      }
       if (c.cap > 0.f) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
@@ -1439,7 +1507,8 @@ attention_dkv_kernel(AttentionCall c) {
       const int64_t at = (int64_t)col[rb].row * c.hk + place.head;
       const int64_t one = (int64_t)c.nk * c.hk * c.d;
       float *piece = c.splits > 1 ? c.part + place.piece * 2 * one : nullptr;
-      store_columns<T, DP, RB, WK>(acc_k, rb, c.dk, piece, at, c.d, c.scale);
+      store_columns<T, DP, RB, WK>(acc_k, rb, c.dk, piece, at, c.d,
+                                   c.cap > 0.f ? c.scale * kFlatUp<T> : c.scale);
       store_columns<T, DP, RB, WK>(acc_v, rb, c.dv, piece ? piece + one : nullptr,
                                    at, c.d, 1.f / kWeightUp<T>);
     }
@@ -1448,36 +1517,31 @@ attention_dkv_kernel(AttentionCall c) {
 // ---- launch -------------------------------------------------------------------
 
 template <typename T, int DP>
-hipError_t launch(const AttentionCall &c, int pass, bool wide,
+hipError_t launch(const AttentionCall &c, int pass, int rows,
                   hipStream_t stream) {
   const int64_t owned =
       pass == 2 ? c.nk : (int64_t)c.nq * (c.hq / c.hk);
-  const int rows = wide ? wide_rows(pass, sizeof(T), DP) : kFewRows;
   const int64_t grid = (owned + rows - 1) / rows * c.hk * c.splits;
   if (grid <= 0)
     return hipSuccess;
   if (grid > INT32_MAX)
     return hipErrorInvalidValue;
   const dim3 g((unsigned)grid), b(kThreads);
+#define PCA_LAUNCH(kernel, most)                                               \
+  if (rows == kFewRows)                                                        \
+    kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);                               \
+  else if (rows == 64)                                                         \
+    kernel<T, DP, 1, 1><<<g, b, 0, stream>>>(c);                               \
+  else                                                                         \
+    kernel<T, DP, most / 64, 1><<<g, b, 0, stream>>>(c)
   if (pass == 0) {
-    if (wide)
-      attention_forward_kernel<T, DP, wide_rows(0, sizeof(T), DP) / 64, 1>
-          <<<g, b, 0, stream>>>(c);
-    else
-      attention_forward_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
+    PCA_LAUNCH(attention_forward_kernel, most_rows(0, sizeof(T), DP));
   } else if (pass == 1) {
-    if (wide)
-      attention_dq_kernel<T, DP, wide_rows(1, sizeof(T), DP) / 64, 1>
-          <<<g, b, 0, stream>>>(c);
-    else
-      attention_dq_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
+    PCA_LAUNCH(attention_dq_kernel, most_rows(1, sizeof(T), DP));
   } else {
-    if (wide)
-      attention_dkv_kernel<T, DP, wide_rows(2, sizeof(T), DP) / 64, 1>
-          <<<g, b, 0, stream>>>(c);
-    else
-      attention_dkv_kernel<T, DP, 1, 4><<<g, b, 0, stream>>>(c);
+    PCA_LAUNCH(attention_dkv_kernel, most_rows(2, sizeof(T), DP));
   }
+#undef PCA_LAUNCH
   return hipGetLastError();
 }
 

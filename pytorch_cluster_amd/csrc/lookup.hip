@@ -7,7 +7,7 @@
 // gradient (places that a search left empty hold -1).
 //
 // The gradient is summed in 32 bits without atomics: the entries are sorted by index,
-// stable and by digits of up to 8 bits (entries of no row come last), and the sorted
+// stable and by digits of up to 10 bits (entries of no row come last), and the sorted
 // list is cut into chunks of equal length whatever the rows are -- one row may have most
 // entries.  A group of lanes adds up a chunk, run after run; a run that lies in one
 // chunk goes straight to the gradient, the others leave their first and last sums in
@@ -23,9 +23,11 @@ namespace pca {
 
 namespace {
 
-constexpr int kSortThreads = 512, kPer = 8;
+constexpr int kSortThreads = 1024, kPer = 4;
 constexpr int kTile = kSortThreads * kPer; // entries of a sorting workgroup
-constexpr int kBits = 8, kDigits = 1 << kBits;
+// (1,024 digits, a thread each: two passes for tables of up to a million rows)
+constexpr int kBits = 10, kDigits = 1 << kBits;
+static_assert(kDigits == kSortThreads, "a thread for each digit");
 
 size_t lk_align(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -41,36 +43,63 @@ __device__ __forceinline__ uint32_t key_at(const LookupCall &c, int64_t e) {
 
 // ---- forward ------------------------------------------------------------------
 
-// A thread per 16 bytes of an output row.
-template <typename T>
-__global__ __launch_bounds__(256) void
-lookup_kernel(LookupCall c, int64_t pieces, int64_t total) {
+// A thread takes kAhead pieces of 16 bytes of output rows, kAhead reads of indices and
+// then of rows in flight.
+constexpr int kAhead = 4;
+
+// I: what counts pieces (32 bits where they suffice: the division by the pieces of a row
+// is most of the arithmetic).
+template <typename T, typename I>
+__global__ __launch_bounds__(256) void lookup_kernel(LookupCall c, I pieces,
+                                                     I total) {
   constexpr int PER = 16 / (int)sizeof(T);
-  for (int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x; at < total;
-       at += (int64_t)gridDim.x * 256) {
-    const int64_t e = at / pieces;
-    const int64_t e0 = (at - e * pieces) * PER;
-    const int64_t row = index_at(c, e);
-    T v[PER];
+  const I first = (I)blockIdx.x * (256 * kAhead) + threadIdx.x;
+  I e[kAhead], e0[kAhead];
+  int64_t row[kAhead];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    const I at = min(first + k * 256, total - 1);
+    e[k] = at / pieces;
+    e0[k] = (at - e[k] * pieces) * PER;
+    row[k] = index_at(c, (int64_t)e[k]);
+  }
+  T v[kAhead][PER];
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
 #pragma unroll
     for (int i = 0; i < PER; ++i)
-      v[i] = (T)0.f;
-    const bool there = row >= 0 && row < c.table;
-    const T *from = static_cast<const T *>(c.rows) + row * c.width + e0;
-    T *to = static_cast<T *>(c.out) + e * c.width + e0;
-    if (c.width % PER == 0) {
-      if (there) {
-        __builtin_memcpy(v, __builtin_assume_aligned(from, 16), 16);
+      v[k][i] = (T)0.f;
+    if (row[k] >= 0 && row[k] < c.table) {
+      const T *from = static_cast<const T *>(c.rows) + row[k] * c.width + e0[k];
+      if (c.width % PER == 0) {
+        __builtin_memcpy(v[k], __builtin_assume_aligned(from, 16), 16);
+      } else {
 #pragma unroll
         for (int i = 0; i < PER; ++i)
-          v[i] = (T)((float)v[i] * c.scale);
+          if ((int64_t)e0[k] + i < c.width)
+            v[k][i] = from[i];
       }
-      __builtin_memcpy(__builtin_assume_aligned(to, 16), v, 16);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    if (first + k * 256 >= total)
+      break;
+    T *to = static_cast<T *>(c.out) + (int64_t)e[k] * c.width + e0[k];
+    const bool there = row[k] >= 0 && row[k] < c.table;
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      v[k][i] = there ? (T)((float)v[k][i] * c.scale) : (T)0.f;
+    if (c.width % PER == 0) {
+      // (written once and read by nobody here: the caches stay with the table)
+      attn::u32x4 o;
+      __builtin_memcpy(&o, v[k], 16);
+      __builtin_nontemporal_store(o, reinterpret_cast<attn::u32x4 *>(to));
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (e0 + i < c.width)
-          to[i] = there ? (T)((float)from[i] * c.scale) : (T)0.f;
+        if ((int64_t)e0[k] + i < c.width)
+          to[i] = v[k][i];
     }
   }
 }
@@ -97,20 +126,30 @@ __device__ __forceinline__ uint64_t pair_at(const LookupCall &c,
   return (p.number & 1 ? s.a : s.b)[e];
 }
 
+// Zeros to the gradient, by workgroups `block` of `blocks`: `clear` bytes from 16-byte
+// bounds on.
+__device__ __forceinline__ void clear_rows(void *out, int64_t clear, int block,
+                                           int blocks) {
+  const int64_t whole = clear / 16;
+  for (int64_t i = (int64_t)block * kSortThreads + threadIdx.x; i < whole;
+       i += (int64_t)blocks * kSortThreads)
+    static_cast<uint4 *>(out)[i] = make_uint4(0, 0, 0, 0);
+  if (block == 0 && threadIdx.x < (clear % 16) / 2)
+    static_cast<uint16_t *>(out)[whole * 8 + threadIdx.x] = 0;
+}
+
 // Entries of a tile by digit; in the first pass the whole grid also clears the
 // gradient (rows without entries keep the zeros).
 __global__ __launch_bounds__(kSortThreads) void
 lookup_count_kernel(LookupCall c, Sorted s, Pass p, int64_t clear) {
   __shared__ uint32_t count[kDigits];
   const int tid = threadIdx.x;
-  for (int64_t i = (int64_t)blockIdx.x * kSortThreads + tid; i < clear;
-       i += (int64_t)gridDim.x * kSortThreads)
-    static_cast<uint16_t *>(c.out)[i] = 0;
+  if (clear > 0)
+    clear_rows(c.out, clear, blockIdx.x, gridDim.x);
   const int tile = blockIdx.x;
   if (tile >= s.tiles)
     return;
-  if (tid < kDigits)
-    count[tid] = 0u;
+  count[tid] = 0u;
   __syncthreads();
   const uint32_t mask = (1u << p.bits) - 1;
 #pragma unroll
@@ -122,7 +161,7 @@ lookup_count_kernel(LookupCall c, Sorted s, Pass p, int64_t clear) {
                 1u);
   }
   __syncthreads();
-  if (tid < kDigits)
+  if (tid < 1 << p.bits)
     s.digits[(size_t)tid * s.tiles + tile] = count[tid];
 }
 
@@ -202,19 +241,16 @@ rank_tile(const uint64_t (&v)[kPer], int mine, int some, int shift, int bits,
   }
   __syncthreads();
   uint32_t count = 0, total;
-  if (tid < kDigits)
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w)
-      count += place[w][tid];
+  for (int w = 0; w < WAVES; ++w)
+    count += place[w][tid];
   local = prefix(count, part, total);
-  if (tid < kDigits) {
-    uint32_t run = local;
+  uint32_t run = local;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const uint32_t n = place[w][tid];
-      place[w][tid] = run;
-      run += n;
-    }
+  for (int w = 0; w < WAVES; ++w) {
+    const uint32_t n = place[w][tid];
+    place[w][tid] = run;
+    run += n;
   }
   __syncthreads();
 }
@@ -237,7 +273,7 @@ lookup_scatter_kernel(LookupCall c, Sorted s, Pass p) {
     v[i] = pair_at(c, s, p, first + min(mine + i * 64, some - 1));
   // what is before the digit's entries: of smaller digits, in the tiles before
   uint32_t offset = 0, all = 0, total;
-  if (tid < kDigits) {
+  if (tid < 1 << p.bits) {
     offset = s.digits[(size_t)tid * s.tiles + blockIdx.x];
     all = s.digits[(size_t)kDigits * s.tiles + tid];
   }
@@ -251,8 +287,7 @@ lookup_scatter_kernel(LookupCall c, Sorted s, Pass p) {
       lds[place[wave][digit] + rank[i]] = v[i];
   }
   __syncthreads();
-  if (tid < kDigits)
-    place[0][tid] = offset - local; // (modulo 2^32)
+  place[0][tid] = offset - local; // (modulo 2^32)
   __syncthreads();
   uint64_t *out = p.number & 1 ? s.b : s.a;
 #pragma unroll
@@ -283,9 +318,7 @@ lookup_small_sort_kernel(LookupCall c, Sorted s, int bits, int64_t clear) {
   __shared__ uint32_t part[kSortThreads / 64];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (blockIdx.x > 0) {
-    for (int64_t i = (int64_t)(blockIdx.x - 1) * kSortThreads + tid; i < clear;
-         i += (int64_t)(gridDim.x - 1) * kSortThreads)
-      static_cast<uint16_t *>(c.out)[i] = 0;
+    clear_rows(c.out, clear, blockIdx.x - 1, gridDim.x - 1);
     return;
   }
   const int some = (int)c.entries;
@@ -369,15 +402,22 @@ lookup_sum_kernel(LookupCall c, Sorted s, Chunks k) {
           to[i] = (T)(sum[i] * c.scale);
     }
   };
+  // the next entries' keys and numbers are read while their predecessors' rows are
+  // under way
+  uint32_t key[AHEAD], perm[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    const int64_t e = min(begin + j, end - 1);
+    key[j] = s.keys[e];
+    perm[j] = s.perm[e];
+  }
   for (int64_t at = begin; at < end; at += AHEAD) {
     T v[AHEAD][PER];
-    uint32_t key[AHEAD];
+    uint32_t next_key[AHEAD], next_perm[AHEAD];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-      const int64_t e = min(at + j, end - 1);
-      key[j] = s.keys[e];
       const T *from =
-          static_cast<const T *>(c.rows) + (int64_t)s.perm[e] * c.width + e0;
+          static_cast<const T *>(c.rows) + (int64_t)perm[j] * c.width + e0;
       if (vec) {
         __builtin_memcpy(v[j], __builtin_assume_aligned(from, 16), 16);
       } else {
@@ -385,6 +425,12 @@ lookup_sum_kernel(LookupCall c, Sorted s, Chunks k) {
         for (int i = 0; i < PER; ++i)
           v[j][i] = e0 + i < c.width ? from[i] : (T)0.f;
       }
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int64_t e = min(at + AHEAD + j, end - 1);
+      next_key[j] = s.keys[e];
+      next_perm[j] = s.perm[e];
     }
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
@@ -404,67 +450,119 @@ lookup_sum_kernel(LookupCall c, Sorted s, Chunks k) {
       for (int i = 0; i < PER; ++i)
         sum[i] += (float)v[j][i];
     }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      key[j] = next_key[j];
+      perm[j] = next_perm[j];
+    }
   }
   put(end < c.entries && s.keys[end] == now);
 }
 
-// A workgroup per chunk in which a run starts that goes on behind it: the run's parts,
-// dealt to the groups of lanes and put together in the order of the groups.
+// A group of lanes per chunk: where a run starts in it that goes on behind it, the run's
+// parts are added up.  Runs of many chunks (kLong or more) are added up by the whole
+// workgroup, one after the other: parts dealt to the groups, put together in the order
+// of the groups.
+constexpr int kLong = 16;
+
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void
 lookup_join_kernel(LookupCall c, Sorted s, Chunks k) {
   constexpr int PER = 16 / (int)sizeof(T), GROUPS = 256 / LANES;
   __shared__ float part[GROUPS][LANES * PER + 1];
-  __shared__ int64_t after_last;
-  const int64_t chunk = blockIdx.x;
-  const int64_t begin = chunk * k.length;
-  const int64_t end = min(begin + k.length, c.entries);
-  if (end >= c.entries)
-    return;
-  const uint32_t now = s.keys[end - 1];
-  if (now == (uint32_t)c.table || s.keys[end] != now ||
-      (s.keys[begin] == now && begin > 0 && s.keys[begin - 1] == now))
-    return;
-  // chunks behind this one that begin with the run's row
-  if (threadIdx.x == 0) {
-    int64_t lo = chunk + 1, hi = k.count;
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) >> 1;
-      if (s.keys[mid * k.length] == now)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    after_last = hi;
-  }
-  __syncthreads();
-  const int64_t stop = after_last;
+  __shared__ int64_t long_stop[GROUPS];
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const int64_t e0 = ((int64_t)blockIdx.y * LANES + lane) * PER;
-  float sum[PER];
+  auto row_of = [&](int64_t chunk) {
+    return s.keys[min((chunk + 1) * k.length, c.entries) - 1];
+  };
+  const bool vec = c.width % PER == 0 && e0 < c.width;
+  auto add = [&](float (&sum)[PER], int64_t chunk, int64_t at) {
+    const float *from = k.ends + (at * 2 + (at == chunk ? 1 : 0)) * c.width + e0;
+    if (vec) {
+      float v[PER];
+      __builtin_memcpy(v, __builtin_assume_aligned(from, 16), sizeof(v));
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    sum[i] = 0.f;
-  for (int64_t at = chunk + grp; at < stop; at += GROUPS) {
-    const float *from =
-        k.ends + (at * 2 + (at == chunk ? 1 : 0)) * c.width + e0;
+      for (int i = 0; i < PER; ++i)
+        sum[i] += v[i];
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       if (e0 + i < c.width)
         sum[i] += from[i];
-  }
+  };
+  {
+    const int64_t chunk = (int64_t)blockIdx.x * GROUPS + grp;
+    const int64_t begin = chunk * k.length, end = begin + k.length;
+    int64_t stop = 0; // first chunk behind the run; 0: none starts here
+    if (end < c.entries) {
+      const uint32_t now = s.keys[end - 1];
+      if (now != (uint32_t)c.table && s.keys[end] == now &&
+          !(s.keys[begin] == now && begin > 0 && s.keys[begin - 1] == now)) {
+        // chunks behind this one that begin with the run's row
+        int64_t lo = chunk + 1, hi = k.count;
+        for (int64_t step = 1; lo + step < hi; step *= 2) {
+          if (s.keys[(lo + step) * k.length] != now) {
+            hi = lo + step;
+            break;
+          }
+          lo += step;
+        }
+        while (hi - lo > 1) {
+          const int64_t mid = (lo + hi) >> 1;
+          if (s.keys[mid * k.length] == now)
+            lo = mid;
+          else
+            hi = mid;
+        }
+        stop = hi;
+        if (stop - chunk < kLong && e0 < c.width) {
+          float sum[PER];
 #pragma unroll
-  for (int i = 0; i < PER; ++i)
-    part[grp][lane * PER + i] = sum[i];
+          for (int i = 0; i < PER; ++i)
+            sum[i] = 0.f;
+          for (int64_t at = chunk; at < stop; ++at)
+            add(sum, chunk, at);
+          T *to = static_cast<T *>(c.out) + (int64_t)now * c.width + e0;
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            if (e0 + i < c.width)
+              to[i] = (T)(sum[i] * c.scale);
+        }
+      }
+    }
+    if (lane == 0)
+      long_stop[grp] = stop - chunk >= kLong ? stop : 0;
+  }
   __syncthreads();
-  for (int col = threadIdx.x; col < LANES * PER; col += 256) {
-    const int64_t e = (int64_t)blockIdx.y * LANES * PER + col;
-    if (e >= c.width)
-      continue;
-    float all = 0.f;
-    for (int g = 0; g < GROUPS; ++g)
-      all += part[g][col];
-    static_cast<T *>(c.out)[(int64_t)now * c.width + e] = (T)(all * c.scale);
+  for (int g = 0; g < GROUPS; ++g) {
+    const int64_t stop = long_stop[g];
+    if (stop == 0)
+      continue; // (the whole workgroup)
+    const int64_t chunk = (int64_t)blockIdx.x * GROUPS + g;
+    float sum[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      sum[i] = 0.f;
+#pragma unroll 8
+    for (int64_t at = chunk + grp; at < stop; at += GROUPS)
+      add(sum, chunk, at);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      part[grp][lane * PER + i] = sum[i];
+    __syncthreads();
+    for (int col = threadIdx.x; col < LANES * PER; col += 256) {
+      const int64_t e = (int64_t)blockIdx.y * LANES * PER + col;
+      if (e >= c.width)
+        continue;
+      float all = 0.f;
+      for (int j = 0; j < GROUPS; ++j)
+        all += part[j][col];
+      static_cast<T *>(c.out)[(int64_t)row_of(chunk) * c.width + e] =
+          (T)(all * c.scale);
+    }
   }
 }
 
@@ -477,7 +575,7 @@ int bit_length(uint64_t v) {
 
 Chunks chunks_of(int64_t entries) {
   Chunks k;
-  k.length = std::clamp<int64_t>((entries + 8191) / 8192, 16, 1 << 20);
+  k.length = std::clamp<int64_t>((entries + 32767) / 32768, 16, 1 << 20);
   k.count = (entries + k.length - 1) / k.length;
   k.ends = nullptr;
   return k;
@@ -493,7 +591,8 @@ void launch_sums(const LookupCall &c, const Sorted &s, const Chunks &k,
       <<<dim3((unsigned)((k.count + GROUPS - 1) / GROUPS), columns), dim3(256),
          0, stream>>>(c, s, k);
   lookup_join_kernel<T, LANES>
-      <<<dim3((unsigned)k.count, columns), dim3(256), 0, stream>>>(c, s, k);
+      <<<dim3((unsigned)((k.count + GROUPS - 1) / GROUPS), columns), dim3(256),
+         0, stream>>>(c, s, k);
 }
 
 template <typename T>
@@ -517,9 +616,15 @@ template <typename T>
 hipError_t launch_forward(const LookupCall &c, hipStream_t stream) {
   const int64_t pieces = (c.width * (int64_t)sizeof(T) + 15) / 16;
   const int64_t total = pieces * c.entries;
-  const int64_t blocks = std::min<int64_t>((total + 255) / 256, 1 << 16);
-  lookup_kernel<T>
-      <<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(c, pieces, total);
+  const int64_t blocks = (total + 256 * kAhead - 1) / (256 * kAhead);
+  if (blocks > INT32_MAX)
+    return hipErrorInvalidValue;
+  if (total < (1ll << 31))
+    lookup_kernel<T, uint32_t><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
+        c, (uint32_t)pieces, (uint32_t)total);
+  else
+    lookup_kernel<T, int64_t><<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
+        c, pieces, total);
   return hipGetLastError();
 }
 
@@ -565,11 +670,11 @@ hipError_t lookup_backward(const LookupCall &c, int dtype, void *workspace,
       reinterpret_cast<uint32_t *>(take(4 * (size_t)kDigits * (tiles + 1)));
   k.ends = reinterpret_cast<float *>(take(8 * (size_t)k.count * c.width));
   const int64_t clear =
-      c.table * c.width * (int64_t)(element_size(dtype) / 2);
+      c.table * c.width * (int64_t)element_size(dtype); // bytes
   const int bits = bit_length((uint64_t)c.table);
   if (c.entries <= kTile) {
     const int64_t fill = std::min<int64_t>(
-        (clear + kSortThreads * 8 - 1) / (kSortThreads * 8), 2048);
+        (clear + kSortThreads * 64 - 1) / (kSortThreads * 64), 2048);
     Sorted one = s;
     LookupCall some = c;
     lookup_small_sort_kernel<<<dim3((unsigned)(1 + fill)), dim3(kSortThreads),
@@ -587,12 +692,13 @@ hipError_t lookup_backward(const LookupCall &c, int dtype, void *workspace,
       p.last = n == passes - 1;
       const int64_t fill =
           n == 0 ? std::min<int64_t>(
-                       (clear + kSortThreads * 8 - 1) / (kSortThreads * 8), 2048)
+                       (clear + kSortThreads * 64 - 1) / (kSortThreads * 64), 2048)
                  : 0;
       lookup_count_kernel<<<dim3((unsigned)std::max<int64_t>(tiles, fill)),
                             dim3(kSortThreads), 0, stream>>>(
           c, s, p, n == 0 ? clear : 0);
-      lookup_scan_kernel<<<dim3(kDigits), dim3(kSortThreads), 0, stream>>>(s);
+      lookup_scan_kernel<<<dim3(1u << p.bits), dim3(kSortThreads), 0, stream>>>(
+          s);
       lookup_scatter_kernel<<<dim3((unsigned)tiles), dim3(kSortThreads), 0,
                               stream>>>(c, s, p);
     }

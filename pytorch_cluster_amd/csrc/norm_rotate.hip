@@ -26,12 +26,36 @@ namespace pca {
 namespace {
 
 constexpr int kRowThreads = 256;
-constexpr int kRowBlocks = 1024; // workgroups of the backward pass, at most
+constexpr int kRowBlocks = 1024; // workgroups, at most: four to a CU
 
-__device__ __forceinline__ float weight_at(const void *w, int dtype, int e) {
-  return dtype == 0   ? static_cast<const float *>(w)[e]
-         : dtype == 2 ? (float)static_cast<const _Float16 *>(w)[e]
-                      : (float)static_cast<const __bf16 *>(w)[e];
+// Elements e0, e0 + 1, ... of a weight, ones if there is none (behind d: something).  One
+// branch on the type for all of them, so that their loads are under way together.
+template <int PER>
+__device__ __forceinline__ void load_weight(float (&w)[PER], const void *p,
+                                            int dtype, int e0, int d) {
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    w[i] = 1.f;
+  if (p == nullptr)
+    return;
+  int at[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    at[i] = min(e0 + i, d - 1);
+  if (dtype == 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      w[i] = static_cast<const float *>(p)[at[i]];
+  } else {
+    uint16_t v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      v[i] = static_cast<const uint16_t *>(p)[at[i]];
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      w[i] = dtype == 2 ? (float)__builtin_bit_cast(_Float16, v[i])
+                        : __uint_as_float((uint32_t)v[i] << 16);
+  }
 }
 
 __device__ __forceinline__ int padded(int e) { return e + (e >> 3); }
@@ -60,68 +84,53 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// Rotates the PER elements from e0 that the lane holds (of a row in `line`).
-template <int PER>
-__device__ __forceinline__ void turn(float (&y)[PER], float *line, int e0,
-                                     int d, int rotated, const float (&cs)[PER],
-                                     const float (&sn)[PER]) {
-#pragma unroll
-  for (int i = 0; i < PER; ++i)
-    if (e0 + i < d)
-      line[padded(e0 + i)] = y[i];
-  wave_fence();
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int e = e0 + i;
-    if (e < 2 * rotated) {
-      const int other = e < rotated ? e + rotated : e - rotated;
-      y[i] = fmaf(line[padded(other)], sn[i], y[i] * cs[i]);
-    }
-  }
-  wave_fence();
-}
-
-// LANES lanes a row.  `heads_each`: heads that a group takes (side 0's, then side 1's).
+// LANES lanes a row.  A workgroup takes heads [blockIdx.y heads_each, ...) (side 0's, then
+// side 1's) of its rows, HEADS at a time, whose chains of dependent steps -- sums across
+// lanes, the exchange in LDS -- overlap; the next ones' loads are under way meanwhile.
+// Which head it is is the same in every lane: bases, strides and weights are picked by
+// the scalar unit.
 template <typename T, int LANES, bool BACKWARD>
-__global__ __launch_bounds__(kRowThreads) void
+__global__ __launch_bounds__(kRowThreads, BACKWARD ? 3 : 4) void
 norm_rotate_kernel(NormRotateCall c, int heads_each) {
   constexpr int PER = 16 / (int)sizeof(T), DP = PER * LANES;
+  constexpr int HEADS = BACKWARD && PER == 8 ? 1 : 2; // (as many as the registers hold)
   constexpr int LINE = DP + DP / 8 + 1;
   constexpr int GROUPS = kRowThreads / LANES;
-  __shared__ float line[GROUPS][LINE];
+  __shared__ float line[GROUPS][HEADS][LINE];
   __shared__ float angle[GROUPS][2][DP / 2 + DP / 16 + 1];
   const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
   const int e0 = lane * PER;
-  const int heads = c.side[0].heads + c.side[1].heads;
-  const int parts = (heads + heads_each - 1) / heads_each;
+  const int head0 = blockIdx.y * heads_each;
+  const int stop = min(head0 + heads_each, c.side[0].heads + c.side[1].heads);
+  const float per_d = 1.f / (float)c.d;
   float w[2][PER], dw[2][PER];
+  int other[PER]; // where an element's partner lies; its own place if it has none
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int e = e0 + i;
+    other[i] = padded(e < c.rotated       ? e + c.rotated
+                      : e < 2 * c.rotated ? e - c.rotated
+                                          : e);
+    dw[0][i] = dw[1][i] = 0.f;
+  }
 #pragma unroll
   for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      w[s][i] = 1.f;
-      dw[s][i] = 0.f;
-      if (c.side[s].weight && e0 + i < c.d)
-        w[s][i] = weight_at(c.side[s].weight, c.weight_dtype, e0 + i);
-    }
+    load_weight<PER>(w[s], c.side[s].weight, c.weight_dtype, e0, c.d);
 
-  const int64_t items = (int64_t)c.rows * parts;
-  for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < items;
+  for (int64_t first = (int64_t)blockIdx.x * GROUPS; first < c.rows;
        first += (int64_t)gridDim.x * GROUPS) {
-    const int64_t item = first + grp;
-    const bool there = item < items; // (lanes of a group agree)
-    const int64_t row = there ? item / parts : 0;
-    const int head0 = there ? (int)(item % parts) * heads_each : 0;
+    // (groups behind the last row repeat it and write nothing)
+    const bool there = first + grp < c.rows;
+    const int64_t row = there ? first + grp : c.rows - 1;
     float cs[PER], sn[PER];
-    if (there)
-      row_angles(c, row, lane, LANES, angle[grp][0], angle[grp][1]);
+    row_angles(c, row, lane, LANES, angle[grp][0], angle[grp][1]);
     wave_fence();
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int e = e0 + i;
       cs[i] = 1.f;
       sn[i] = 0.f;
-      if (there && e < 2 * c.rotated) {
+      if (e < 2 * c.rotated) {
         const int r = e < c.rotated ? e : e - c.rotated;
         cs[i] = angle[grp][0][padded(r)];
         sn[i] = angle[grp][1][padded(r)];
@@ -131,89 +140,156 @@ norm_rotate_kernel(NormRotateCall c, int heads_each) {
       }
     }
     wave_fence();
-    const int stop = there ? min(head0 + heads_each, heads) : 0;
-    for (int h = head0; h < stop; ++h) {
-      const int s = h < c.side[0].heads ? 0 : 1;
+
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
       const NormRotateSide &side = c.side[s];
-      const int head = s == 0 ? h : h - c.side[0].heads;
-      T raw[PER];
-      float x[PER], sum = 0.f;
-      const attn::u32x4 v =
-          attn::load_piece<T, DP>(side.x, row, head, lane, c.d);
-      __builtin_memcpy(raw, &v, 16);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        x[i] = (float)raw[i];
-        sum = fmaf(x[i], x[i], sum);
-      }
-#pragma unroll
-      for (int sh = 1; sh < LANES; sh <<= 1)
-        sum += __shfl_xor(sum, sh);
-      const float inv = 1.f / __builtin_sqrtf(sum / (float)c.d + c.eps);
-      float y[PER];
-      if constexpr (!BACKWARD) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          y[i] = x[i] * inv * w[s][i];
-        turn<PER>(y, line[grp], e0, c.d, c.rotated, cs, sn);
-      } else {
-        const attn::u32x4 gv =
-            attn::load_piece<T, DP>(side.dout, row, head, lane, c.d);
-        __builtin_memcpy(raw, &gv, 16);
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          y[i] = (float)raw[i];
-        turn<PER>(y, line[grp], e0, c.d, c.rotated, cs, sn);
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          x[i] *= inv;
-          dw[s][i] = fmaf(y[i], x[i], dw[s][i]);
-          y[i] *= w[s][i];
-          dot = fmaf(y[i], x[i], dot);
-        }
-#pragma unroll
-        for (int sh = 1; sh < LANES; sh <<= 1)
-          dot += __shfl_xor(dot, sh);
-        dot /= (float)c.d;
-#pragma unroll
-        for (int i = 0; i < PER; ++i)
-          y[i] = inv * (y[i] - x[i] * dot);
-      }
-      T *out = static_cast<T *>(side.out) +
-               (row * side.heads + head) * (int64_t)c.d + e0;
-      if (c.d % PER == 0) {
-        if (e0 < c.d) {
+      const int before = s == 0 ? 0 : c.side[0].heads;
+      const int begin = max(head0 - before, 0);
+      const int end = min(stop - before, side.heads);
+      const T *const x_row =
+          static_cast<const T *>(side.x.data) + row * side.x.row + e0;
+      const T *const g_row =
+          static_cast<const T *>(side.dout.data) + row * side.dout.row + e0;
+      T *const out_row =
+          static_cast<T *>(side.out) + row * side.heads * c.d + e0;
+      auto load = [&](const T *p, bool vec) {
+        attn::u32x4 r = {0, 0, 0, 0};
+        if (vec) {
+          if (e0 < c.d)
+            r = *reinterpret_cast<const attn::u32x4 *>(p);
+        } else {
+          T e[PER];
 #pragma unroll
           for (int i = 0; i < PER; ++i)
-            raw[i] = (T)y[i];
-          attn::u32x4 o;
-          __builtin_memcpy(&o, raw, 16);
-          *reinterpret_cast<attn::u32x4 *>(out) = o;
+            e[i] = e0 + i < c.d ? p[i] : (T)0.f;
+          __builtin_memcpy(&r, e, 16);
         }
-      } else {
+        return r;
+      };
+      attn::u32x4 next_x[HEADS], next_g[HEADS];
+      auto fetch = [&](int h0) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i)
-          if (e0 + i < c.d)
-            out[i] = (T)y[i];
+        for (int k = 0; k < HEADS; ++k)
+          if (h0 + k < end) {
+            next_x[k] = load(x_row + (h0 + k) * side.x.head, side.x.vec);
+            if constexpr (BACKWARD)
+              next_g[k] =
+                  load(g_row + (h0 + k) * side.dout.head, side.dout.vec);
+          }
+      };
+      fetch(begin);
+      for (int h0 = begin; h0 < end; h0 += HEADS) {
+        T raw[PER];
+        float x[HEADS][PER], y[HEADS][PER], sum[HEADS], inv[HEADS];
+#pragma unroll
+        for (int k = 0; k < HEADS; ++k) {
+          __builtin_memcpy(raw, &next_x[k], 16);
+          sum[k] = 0.f;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            x[k][i] = (float)raw[i];
+            sum[k] = fmaf(x[k][i], x[k][i], sum[k]);
+          }
+          if constexpr (BACKWARD) {
+            __builtin_memcpy(raw, &next_g[k], 16);
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              y[k][i] = (float)raw[i];
+          }
+        }
+        fetch(h0 + HEADS);
+#pragma unroll
+        for (int sh = 1; sh < LANES; sh <<= 1)
+#pragma unroll
+          for (int k = 0; k < HEADS; ++k)
+            sum[k] += __shfl_xor(sum[k], sh);
+#pragma unroll
+        for (int k = 0; k < HEADS; ++k) {
+          inv[k] = __builtin_amdgcn_rsqf(fmaf(sum[k], per_d, c.eps));
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            x[k][i] *= inv[k];
+            if constexpr (!BACKWARD)
+              y[k][i] = x[k][i] * w[s][i];
+            line[grp][k][padded(e0 + i)] = y[k][i];
+          }
+        }
+        wave_fence();
+#pragma unroll
+        for (int k = 0; k < HEADS; ++k)
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            y[k][i] = fmaf(line[grp][k][other[i]], sn[i], y[k][i] * cs[i]);
+        wave_fence();
+        if constexpr (BACKWARD) {
+          float dot[HEADS];
+#pragma unroll
+          for (int k = 0; k < HEADS; ++k) {
+            dot[k] = 0.f;
+            const bool adds = there && h0 + k < end;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              const float a = y[k][i] * x[k][i];
+              dw[s][i] += adds ? a : 0.f;
+              y[k][i] *= w[s][i];
+              dot[k] = fmaf(y[k][i], x[k][i], dot[k]);
+            }
+          }
+#pragma unroll
+          for (int sh = 1; sh < LANES; sh <<= 1)
+#pragma unroll
+            for (int k = 0; k < HEADS; ++k)
+              dot[k] += __shfl_xor(dot[k], sh);
+#pragma unroll
+          for (int k = 0; k < HEADS; ++k) {
+            dot[k] *= per_d;
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              y[k][i] = inv[k] * fmaf(-x[k][i], dot[k], y[k][i]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < HEADS; ++k) {
+          if (h0 + k >= end || !there)
+            break;
+          T *out = out_row + (int64_t)(h0 + k) * c.d;
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            raw[i] = (T)y[k][i];
+          if (c.d % PER == 0) {
+            if (e0 < c.d) {
+              attn::u32x4 o;
+              __builtin_memcpy(&o, raw, 16);
+              __builtin_nontemporal_store(
+                  o, reinterpret_cast<attn::u32x4 *>(out));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+              if (e0 + i < c.d)
+                out[i] = raw[i];
+          }
+        }
       }
     }
   }
 
   if constexpr (BACKWARD) {
     // the workgroup's share of dw: group after group
+    const int64_t at = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       __syncthreads();
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        line[grp][padded(e0 + i)] = dw[s][i];
+        line[grp][0][padded(e0 + i)] = dw[s][i];
       __syncthreads();
       for (int e = threadIdx.x; e < c.d; e += kRowThreads) {
         float sum = 0.f;
         for (int k = 0; k < GROUPS; ++k)
-          sum += line[k][padded(e)];
-        c.part[((int64_t)blockIdx.x * 2 + s) * c.d + e] = sum;
+          sum += line[k][0][padded(e)];
+        c.part[(at * 2 + s) * c.d + e] = sum;
       }
     }
   }
@@ -227,6 +303,7 @@ sum_weights_kernel(NormRotateCall c, int blocks) {
   const int at = blockIdx.x * 16 + col;
   float sum = 0.f;
   if (at < 2 * c.d)
+#pragma unroll 8
     for (int b = stripe; b < blocks; b += 16)
       sum += c.part[(int64_t)b * 2 * c.d + at];
   part[stripe][col] = sum;
@@ -254,19 +331,21 @@ hipError_t launch_rows(const NormRotateCall &c, bool backward, int &blocks,
                        hipStream_t stream) {
   constexpr int GROUPS = kRowThreads / LANES;
   const int heads = c.side[0].heads + c.side[1].heads;
-  // a group takes all heads of a row where the rows alone fill the chip
+  // a workgroup takes all heads of its rows where the rows alone fill the chip
+  const int64_t want = (c.rows + GROUPS - 1) / GROUPS;
   int each = heads;
-  while (each > 1 && (int64_t)c.rows * ((heads + each - 1) / each) / GROUPS < 512)
+  while (each > 1 && want * ((heads + each - 1) / each) < 512)
     each = (each + 1) / 2;
-  const int64_t items = (int64_t)c.rows * ((heads + each - 1) / each);
-  const int64_t want = (items + GROUPS - 1) / GROUPS;
-  blocks = (int)std::min<int64_t>(want, backward ? kRowBlocks : 16384);
+  const int parts = (heads + each - 1) / each;
+  const int most = std::max(1, kRowBlocks / parts);
+  const dim3 grid((unsigned)std::min<int64_t>(want, most), (unsigned)parts);
+  blocks = (int)(grid.x * grid.y);
   if (backward)
     norm_rotate_kernel<T, LANES, true>
-        <<<dim3(blocks), dim3(kRowThreads), 0, stream>>>(c, each);
+        <<<grid, dim3(kRowThreads), 0, stream>>>(c, each);
   else
     norm_rotate_kernel<T, LANES, false>
-        <<<dim3(blocks), dim3(kRowThreads), 0, stream>>>(c, each);
+        <<<grid, dim3(kRowThreads), 0, stream>>>(c, each);
   return hipGetLastError();
 }
 

@@ -195,10 +195,13 @@ def lookup64(weight, index, scale, dout=None):
     # (scale itself goes to fp32, then one product)
     err = {"out": 2 * E * val["out"].abs() + rounded(val["out"], weight.dtype)}
     if dout is not None:
-        g = dout.reshape(flat.numel(), -1).double()[there]
-        grad, size = torch.zeros_like(w64), torch.zeros_like(w64)
-        grad.index_add_(0, rows, g)
-        size.index_add_(0, rows, g.abs())
+        # (on the host: many entries of one row are slow to add on the device)
+        g = dout.reshape(flat.numel(), -1).double()[there].cpu()
+        grad = torch.zeros(w64.shape, dtype=torch.float64)
+        size = torch.zeros_like(grad)
+        grad.index_add_(0, rows.cpu(), g)
+        size.index_add_(0, rows.cpu(), g.abs())
+        grad, size = grad.to(weight.device), size.to(weight.device)
         many = torch.bincount(rows, minlength=n).double()[:, None] + 8
         val["dweight"] = scale * grad
         err["dweight"] = abs(scale) * many * E * size \
