@@ -67,20 +67,21 @@ typedef struct pca_attention_args {
 /* Scratch of the forward (backward = 0) or the backward call (1); 0: sizes not
  * supported. */
 size_t pca_attention_workspace_bytes(int64_t nq, int64_t nk, int32_t hq,
-                                     int32_t hk, int32_t d, int32_t dtype,
-                                     int backward);
+                                     int32_t hk, int32_t d, int backward);
 
-/* out: [nq, hq, d] dense.  lse: [hq, nq] fp32 for the backward pass, or NULL. */
-int pca_attention_forward(const pca_attention_args *args, void *out, float *lse,
-                          void *workspace, size_t workspace_bytes,
+/* out: [nq, hq, d] dense.  For the backward pass: lse, [hq, nq] fp32, and, with
+ * 16-bit types, rest: what rounding took off out, [nq, hq, d]; or NULL. */
+int pca_attention_forward(const pca_attention_args *args, void *out, void *rest,
+                          float *lse, void *workspace, size_t workspace_bytes,
                           void *stream);
 
-/* Gradients of q, k, v (dense, all three are written) from that of out. */
+/* Gradients of q, k, v (dense, all three are written) from that of out.  rest
+ * may be NULL: dq and dk are then less exact (16-bit types). */
 int pca_attention_backward(const pca_attention_args *args, const void *out,
-                           const float *lse, const void *dout, int64_t dout_row,
-                           int64_t dout_head, void *dq, void *dk, void *dv,
-                           void *workspace, size_t workspace_bytes,
-                           void *stream);
+                           const void *rest, const float *lse, const void *dout,
+                           int64_t dout_row, int64_t dout_head, void *dq,
+                           void *dk, void *dv, void *workspace,
+                           size_t workspace_bytes, void *stream);
 
 /*
  * Norm of every head of q and k and rotation by the row's position:

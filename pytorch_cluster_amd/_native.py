@@ -137,13 +137,13 @@ FEATURES_C_ABI = {
     "pca_spans": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp]),
     "pca_attention_workspace_bytes": (
         ctypes.c_size_t, [_i64, _i64, ctypes.c_int32, ctypes.c_int32,
-                          ctypes.c_int32, ctypes.c_int32, ctypes.c_int]),
+                          ctypes.c_int32, ctypes.c_int]),
     "pca_attention_forward": (
-        ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp, _vp, _vp,
+        ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp, _vp, _vp, _vp,
                        ctypes.c_size_t, _vp]),
     "pca_attention_backward": (
-        ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp, _vp, _vp, _i64, _i64,
-                       _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+        ctypes.c_int, [ctypes.POINTER(AttentionArgs), _vp, _vp, _vp, _vp, _i64,
+                       _i64, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
     "pca_norm_rotate_forward": (
         ctypes.c_int, [ctypes.POINTER(NormRotateArgs), _vp, _vp, _vp]),
     "pca_norm_rotate_workspace_bytes": (ctypes.c_size_t,

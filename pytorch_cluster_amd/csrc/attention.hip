@@ -97,18 +97,18 @@ __global__ __launch_bounds__(256) void spans_kernel(const int64_t *ids_a, int na
   spans[i] = v;
 }
 
+// Writes v rounded to T; returns what that takes off.
 template <typename T>
-__device__ __forceinline__ void put(void *out, int64_t at, float v) {
-  static_cast<T *>(out)[at] = (T)v;
+__device__ __forceinline__ float put(void *out, int64_t at, float v) {
+  const T r = (T)v;
+  static_cast<T *>(out)[at] = r;
+  return v - (float)r;
 }
-__device__ __forceinline__ void put_as(int dtype, void *out, int64_t at,
-                                       float v) {
-  if (dtype == 0)
-    put<float>(out, at, v);
-  else if (dtype == 2)
-    put<_Float16>(out, at, v);
-  else
-    put<__bf16>(out, at, v);
+__device__ __forceinline__ float put_as(int dtype, void *out, int64_t at,
+                                        float v) {
+  return dtype == 0   ? put<float>(out, at, v)
+         : dtype == 2 ? put<_Float16>(out, at, v)
+                      : put<__bf16>(out, at, v);
 }
 
 // Output rows from the pieces' sums, maxima and sums of weights: 32 lanes take four
@@ -125,6 +125,7 @@ join_forward_kernel(AttentionCall c, int dtype, int shares) {
   float top = -__builtin_inff(), sum = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   if (there) {
+#pragma unroll 8
     for (int s = share; s < c.splits; s += shares)
       top = fmaxf(top, c.part_ml[(s * rows + row) * 2]);
 #pragma unroll 4
@@ -181,8 +182,12 @@ join_forward_kernel(AttentionCall c, int dtype, int shares) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 4; ++e)
-    if (e0 + e < c.d)
-      put_as(dtype, c.out, row * c.d + e0 + e, acc[e] * inv);
+    if (e0 + e < c.d) {
+      const int64_t at = row * c.d + e0 + e;
+      const float left = put_as(dtype, c.out, at, acc[e] * inv);
+      if (c.rest)
+        put_as(dtype, c.rest, at, left);
+    }
   if (e0 == 0 && c.lse) {
     const int64_t query = row / c.hq, head = row % c.hq;
     c.lse[head * c.nq + query] =
@@ -190,19 +195,22 @@ join_forward_kernel(AttentionCall c, int dtype, int shares) {
   }
 }
 
-// out[i] = sum over the pieces, in their order.
-__global__ __launch_bounds__(256) void join_sum_kernel(const float *part,
-                                                       int pieces,
-                                                       int64_t stride,
-                                                       int64_t count, int dtype,
-                                                       void *out) {
+// Sums over the pieces, in their order: the first `count` to out, the next ones to
+// `second`.
+__global__ __launch_bounds__(256) void
+join_sum_kernel(const float *part, int pieces, int64_t stride, int64_t count,
+                int dtype, void *out, void *second) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= count)
+  if (i >= stride)
     return;
   float v = 0.f;
+#pragma unroll 4
   for (int s = 0; s < pieces; ++s)
     v += part[s * stride + i];
-  put_as(dtype, out, i, v);
+  if (i < count)
+    put_as(dtype, out, i, v);
+  else
+    put_as(dtype, second, i - count, v);
 }
 
 AttentionLauncher launcher(int dtype, int d) {
@@ -214,26 +222,26 @@ AttentionLauncher launcher(int dtype, int d) {
 #undef PCA_BY_WIDTH
 }
 
-hipError_t join_sum(const AttentionCall &c, const float *part, int64_t stride,
-                    int64_t count, int dtype, void *out, hipStream_t stream) {
-  const int64_t blocks = (count + 255) / 256;
+hipError_t join_sum(const AttentionCall &c, int64_t stride, int64_t count,
+                    int dtype, void *out, void *second, hipStream_t stream) {
+  const int64_t blocks = (stride + 255) / 256;
   if (blocks > INT32_MAX)
     return hipErrorInvalidValue;
   join_sum_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
-      part, c.splits, stride, count, dtype, out);
+      c.part, c.splits, stride, count, dtype, out, second);
   return hipGetLastError();
 }
 
 } // namespace
 
 AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
-                             int dtype, int d) {
+                             int d) {
   const int64_t rows_q = nq * (hq / hk);
   const int64_t owned = pass == 2 ? nk : rows_q;
   const int64_t looped = pass == 2 ? rows_q : nk;
   auto groups = [&](int rows) { return (owned + rows - 1) / rows * hk; };
   AttentionPlan p;
-  p.rows = most_rows(pass, dtype == 0 ? 4 : 2, d);
+  p.rows = most_rows(pass, d);
   if (d <= 32 || (d <= 64 && pass != 2) || groups(p.rows) < 512)
     p.rows = 64;
   if (owned <= 256)
@@ -246,8 +254,8 @@ AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
 }
 
 static size_t part_bytes(int pass, int64_t nq, int64_t nk, int hq, int hk,
-                         int dtype, int d) {
-  const int splits = attention_plan(pass, nq, nk, hq, hk, dtype, d).splits;
+                         int d) {
+  const int splits = attention_plan(pass, nq, nk, hq, hk, d).splits;
   if (splits <= 1)
     return 0;
   const int64_t one = pass == 2 ? 2 * nk * hk * d : nq * hq * d;
@@ -258,17 +266,18 @@ static size_t part_bytes(int pass, int64_t nq, int64_t nk, int hq, int hk,
 }
 
 size_t attention_workspace_bytes(int pass, int64_t nq, int64_t nk, int hq,
-                                 int hk, int dtype, int d) {
+                                 int hk, int d) {
   if (pass == 0)
-    return 256 + part_bytes(0, nq, nk, hq, hk, dtype, d);
-  return attn_align(sizeof(float) * (size_t)(nq * hq)) + 256 +
-         std::max(part_bytes(1, nq, nk, hq, hk, dtype, d),
-                  part_bytes(2, nq, nk, hq, hk, dtype, d));
+    return 256 + part_bytes(0, nq, nk, hq, hk, d);
+  return 2 * attn_align(sizeof(float) * (size_t)(nq * hq)) +
+         attn_align(sizeof(float) * (size_t)hq) + 256 +
+         std::max(part_bytes(1, nq, nk, hq, hk, d),
+                  part_bytes(2, nq, nk, hq, hk, d));
 }
 
 hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
                              hipStream_t stream) {
-  const AttentionPlan p = attention_plan(0, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
+  const AttentionPlan p = attention_plan(0, c.nq, c.nk, c.hq, c.hk, c.d);
   c.splits = p.splits;
   c.part = static_cast<float *>(workspace);
   c.part_ml = c.part + attn_align(sizeof(float) * (size_t)p.splits * c.nq *
@@ -277,7 +286,11 @@ hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
   hipError_t e = launcher(dtype, c.d)(c, 0, p.rows, stream);
   if (e != hipSuccess || p.splits == 1 || c.nq == 0)
     return e;
-  const int shares = p.splits >= 32 ? 8 : p.splits >= 16 ? 4 : 1;
+  // (rows alone fill the chip: a group a row)
+  const int shares = (int64_t)c.nq * c.hq >= 8192 ? 1
+                     : p.splits >= 32             ? 8
+                     : p.splits >= 4              ? 4
+                                                  : 1;
   const int64_t blocks =
       ((int64_t)c.nq * c.hq + 8 / shares - 1) / (8 / shares);
   join_forward_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
@@ -287,26 +300,28 @@ hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
 
 hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
                               hipStream_t stream) {
-  c.delta = static_cast<float *>(workspace);
-  c.part = c.delta +
-           attn_align(sizeof(float) * (size_t)c.nq * c.hq) / sizeof(float);
-  const AttentionPlan pq = attention_plan(1, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
+  const size_t one =
+      attn_align(sizeof(float) * (size_t)c.nq * c.hq) / sizeof(float);
+  c.minus_delta = static_cast<float *>(workspace);
+  c.base = c.minus_delta + one;
+  c.minus_slope = c.base + one;
+  c.part =
+      c.minus_slope + attn_align(sizeof(float) * (size_t)c.hq) / sizeof(float);
+  const AttentionPlan pq = attention_plan(1, c.nq, c.nk, c.hq, c.hk, c.d);
   c.splits = pq.splits;
   hipError_t e = launcher(dtype, c.d)(c, 1, pq.rows, stream);
   if (e == hipSuccess && c.splits > 1 && c.nq > 0) {
     const int64_t count = (int64_t)c.nq * c.hq * c.d;
-    e = join_sum(c, c.part, count, count, dtype, c.dq, stream);
+    e = join_sum(c, count, count, dtype, c.dq, nullptr, stream);
   }
   if (e != hipSuccess)
     return e;
-  const AttentionPlan pk = attention_plan(2, c.nq, c.nk, c.hq, c.hk, dtype, c.d);
+  const AttentionPlan pk = attention_plan(2, c.nq, c.nk, c.hq, c.hk, c.d);
   c.splits = pk.splits;
   e = launcher(dtype, c.d)(c, 2, pk.rows, stream);
   if (e == hipSuccess && c.splits > 1 && c.nk > 0) {
     const int64_t count = (int64_t)c.nk * c.hk * c.d;
-    e = join_sum(c, c.part, 2 * count, count, dtype, c.dk, stream);
-    if (e == hipSuccess)
-      e = join_sum(c, c.part + count, 2 * count, count, dtype, c.dv, stream);
+    e = join_sum(c, 2 * count, count, dtype, c.dk, c.dv, stream);
   }
   return e;
 }

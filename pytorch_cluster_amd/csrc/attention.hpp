@@ -26,7 +26,9 @@ struct AttentionCall {
   int nq = 0, nk = 0, hq = 0, hk = 0, d = 0;
   float scale = 1.f, cap = 0.f;
 
-  void *out = nullptr; // [nq, hq, d], dense
+  void *out = nullptr;  // [nq, hq, d], dense
+  void *rest = nullptr; // the same: what rounding took off out; or NULL (backward:
+                        // read)
   float *lse = nullptr; // [hq, nq]: log2 of the sum of exp2 of the scores (in
                         // units of log 2); +inf for a row without keys
 
@@ -34,7 +36,9 @@ struct AttentionCall {
   const void *out_in = nullptr;
   HeadRows dout;
   void *dq = nullptr, *dk = nullptr, *dv = nullptr; // dense
-  float *delta = nullptr;                           // [hq, nq]
+  // from the kernel of dq to that of dk and dv: -delta and what the scores are
+  // relative to ([hq, nq]), -slope log2 e ([hq])
+  float *minus_delta = nullptr, *base = nullptr, *minus_slope = nullptr;
 
   // the looped side cut into pieces that meet in a kernel of their own
   int splits = 1;
@@ -70,14 +74,14 @@ PCA_ATTENTION_DECLARE(bf16);
 // many.  Two blocks of 16 columns per wave share every left operand; where the sums of
 // both do not fit the registers of two waves per SIMD it is one.
 constexpr int kFewRows = 16;
-constexpr int most_rows(int pass, int size, int width) {
-  return width > 64 && (pass == 2 || (pass == 1 && size == 4)) ? 64 : 128;
+constexpr int most_rows(int pass, int width) {
+  return width > 64 && pass > 0 ? 64 : 128;
 }
 
 AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
-                             int dtype, int d);
+                             int d);
 size_t attention_workspace_bytes(int pass, int64_t nq, int64_t nk, int hq,
-                                 int hk, int dtype, int d);
+                                 int hk, int d);
 // workspace: of attention_workspace_bytes(0, ...) / (1, ...)
 hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
                              hipStream_t stream);

@@ -9,6 +9,11 @@
 //   dS = P (do_i . v_j - delta_i)   dT = dS (1 - (u / cap)^2)
 //   dq = scale sum_j dT k_j   dk = scale sum_i dT q_i   dv = sum_i P do_i
 //
+// With 16-bit rows the forward pass also leaves what rounding took off o_i (`rest`):
+// an error of delta_i would be the same for all j and add up, where those of P and dT,
+// rounded for the matrix cores, do not.  dq and dk are 1.5 times as far from the exact
+// ones as their own rounding without it (one in two rows with few near keys).
+//
 // Everything a kernel sums over lies along the matrix instruction's contraction and
 // everything it owns along its columns: scores are formed transposed, S^T = K Q^T, so
 // that a lane holds scores of ONE owned row (its column, lane % 16) and four
@@ -87,9 +92,13 @@ template <typename T, int DP> struct Shape {
   static constexpr int FB = KF / 16;           // ... in blocks
   // A tile's rows lie in LDS one after the other, as the loads that bypass the
   // registers leave them.  Piece p of row r is kept at place p ^ turn(r): the same
-  // piece of 16 neighbouring rows then lies on 64 different banks.
+  // piece of 16 neighbouring rows then lies on 64 different banks, and so do, for
+  // 16-bit elements, pairs of pieces of 8 neighbouring rows (turned_operand).
   __device__ __forceinline__ static int turn(int row) {
-    return CH >= 16 ? row & 15 : (row / (16 / CH)) & (CH - 1);
+    constexpr int ROWS = CH >= 16 ? 1 : 16 / CH; // that fill the banks
+    if (SZ == 4)
+      return row / ROWS & (CH >= 16 ? 15 : CH - 1);
+    return (row / ROWS & (CH >= 16 ? 7 : CH / 2 - 1)) << 1 | (row >> 3 & 1);
   }
 };
 
@@ -144,6 +153,15 @@ __device__ __forceinline__ void request4(const void *from, uint32_t lds) {
                : "v"(from), "s"(lds)
                : "memory");
 }
+__device__ __forceinline__ void request4(const void *base, uint32_t offset,
+                                         uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\t"
+               "s_nop 0\n\t"
+               "global_load_lds_dword %0, %1"
+               :
+               : "v"(offset), "s"(base), "s"(lds)
+               : "memory");
+}
 // Everything this wave has requested is in LDS; then everything the others have.
 __device__ __forceinline__ void arrive() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -153,9 +171,10 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
   return (uint32_t)(uintptr_t)p; // (the low half of a generic address)
 }
 
-// Rows of looped tiles of one tensor on their way to LDS: ROWS rows of [begin, end),
-// zeros behind the end.  A row stands for (row / group, head0 + row % group).  Pieces
-// beyond d are left alone: the caller has cleared them.
+// Rows of looped tiles of one head of a tensor on their way to LDS: ROWS rows of [begin,
+// end), zeros behind the end.  Pieces beyond d are left alone: the caller has cleared
+// them.  A whole tile costs a thread nothing but the loads: its offset in a tile never
+// changes, the tile's address is formed by the scalar unit.
 template <typename T, int DP, int ROWS> struct Requests {
   using S = Shape<T, DP>;
   static constexpr int N = ROWS * S::CH / kThreads;      // per thread
@@ -164,57 +183,60 @@ template <typename T, int DP, int ROWS> struct Requests {
   static_assert(ROWS * S::CH % kThreads == 0, "tile does not fill the threads");
   const HeadRows &x;
   int d, wave;
+  uint32_t row_bytes;     // of the vector path
   uint32_t offset[LANES]; // bytes of this thread's first pieces from a tile's row
   bool on[LANES];         // they lie in d
 
   __device__ __forceinline__ Requests(const HeadRows &rows, int width)
-      : x(rows), d(width) {
+      : x(rows), d(width), row_bytes((uint32_t)(rows.row * S::SZ)) {
     wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int l = 0; l < LANES; ++l) {
       const int p = piece(threadIdx.x / S::CH + l * STEP);
-      offset[l] =
-          (uint32_t)((threadIdx.x / S::CH) * x.row * S::SZ) + p * 16;
+      offset[l] = (uint32_t)(threadIdx.x / S::CH) * row_bytes + p * 16;
       on[l] = p * S::PER < d;
     }
   }
   __device__ __forceinline__ static int piece(int row) {
     return threadIdx.x % S::CH ^ S::turn(row);
   }
-  __device__ __forceinline__ void operator()(int begin, int end, int group,
-                                             int head0, char *tile) const {
-    const uint32_t lds = lds_address(tile) + wave * 1024;
-    if (x.vec && group == 1 && begin + ROWS <= end) {
-      const char *base = static_cast<const char *>(x.data) +
-                         ((int64_t)begin * x.row + (int64_t)head0 * x.head) *
-                             S::SZ;
-      const int64_t step = (int64_t)STEP * x.row * S::SZ;
+  __device__ __forceinline__ void operator()(int begin, int end, int head,
+                                             char *tile) const {
+    const char *const first =
+        static_cast<const char *>(x.data) + (int64_t)head * x.head * S::SZ;
+    uint32_t lds = lds_address(tile) + wave * 1024;
+    if (x.vec && begin + ROWS <= end) {
+      const char *from = first + (uint64_t)(uint32_t)begin * row_bytes;
+      if (LANES == 1) {
+        if (on[0])
 #pragma unroll
-      for (int l = 0; l < LANES; ++l)
-        if (on[l]) {
+          for (int e = 0; e < N; ++e)
+            request16(from + (uint64_t)(e * STEP * row_bytes), offset[0],
+                      lds + kWaves * e * 1024);
+      } else {
 #pragma unroll
-          for (int e = l; e < N; e += LANES)
-            request16(base + e * step, offset[l], lds + kWaves * e * 1024);
-        }
+        for (int e = 0; e < N; ++e)
+          if (on[e % LANES])
+            request16(from + (uint64_t)(e * STEP * row_bytes),
+                      offset[e % LANES], lds + kWaves * e * 1024);
+      }
       return;
     }
 #pragma unroll 1
     for (int e = 0; e < N; ++e) {
       const int row = threadIdx.x / S::CH + e * STEP;
-      const int at = begin + row;
-      const int r = group == 1 ? at : at / group;
-      const int head = group == 1 ? head0 : head0 + at - r * group;
       const int p = piece(row);
       if (x.vec) {
-        const T *from = static_cast<const T *>(x.data) + (int64_t)r * x.row +
-                        (int64_t)head * x.head + p * S::PER;
+        const char *from =
+            first + (int64_t)(begin + row) * row_bytes + p * 16;
         if (p * S::PER < d)
-          request16(at < end ? (const void *)from : (const void *)kZeros,
+          request16(begin + row < end ? (const void *)from
+                                      : (const void *)kZeros,
                     lds + kWaves * e * 1024);
       } else {
         u32x4 v = {0, 0, 0, 0};
-        if (at < end)
-          v = load_piece<T, DP>(x, r, head, p, d);
+        if (begin + row < end)
+          v = load_piece<T, DP>(x, begin + row, head, p, d);
         *reinterpret_cast<u32x4 *>(tile + (threadIdx.x + e * kThreads) * 16) =
             v;
       }
@@ -309,13 +331,30 @@ __device__ __forceinline__ void store4(T *p, f32x4 v, int left, bool vec) {
   }
 }
 
+// What rounding the elements of a row to T takes off.
+template <typename T> __device__ __forceinline__ f32x4 rest4(f32x4 v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    v[i] -= (float)(T)v[i];
+  return v;
+}
+
+// Over the four groups of 16 lanes, by exchanges in the vector unit: the two results of
+// a swap of v with itself hold both partners' values.
+template <typename Op>
+__device__ __forceinline__ float across_groups(float v, Op op) {
+  const uint32_t a = __float_as_uint(v);
+  const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const uint32_t b =
+      __float_as_uint(op(__uint_as_float(x[0]), __uint_as_float(x[1])));
+  const auto y = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return op(__uint_as_float(y[0]), __uint_as_float(y[1]));
+}
 __device__ __forceinline__ float across_groups_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
+  return across_groups(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float across_groups_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+  return across_groups(v, [](float a, float b) { return a + b; });
 }
 
 // tanh y for fp32 rows, x = 2 y log2 e: (exp2(x) - 1) / (exp2(x) + 1), and near 0,
@@ -341,17 +380,17 @@ template <int ROWS> struct Spans {
 };
 
 // Collects the spans of owned rows [row0, row0 + ROWS) (row / group is the row that has
-// a span), whole workgroup; `scale`: looped rows per entry of a span, `tile`: of a tile.
+// a span; no spans: all of the looped rows), whole workgroup; `tile`: rows of a tile.
 template <int ROWS>
 __device__ __forceinline__ void
 collect_spans(Spans<ROWS> &s, const int2 *spans, int row0, int rows, int group,
-              int all, int scale, int tile) {
+              int all, int tile) {
   if (spans == nullptr) {
     if (threadIdx.x == 0) {
       s.begin[0] = 0;
-      s.end[0] = all * scale;
+      s.end[0] = all;
       s.first[0] = 0;
-      s.first[1] = (all * scale + tile - 1) / tile;
+      s.first[1] = (all + tile - 1) / tile;
       s.count = 1;
     }
     __syncthreads();
@@ -378,8 +417,8 @@ collect_spans(Spans<ROWS> &s, const int2 *spans, int row0, int rows, int group,
       const unsigned long long heads = __ballot(head);
       if (head) {
         const int at = count + __popcll(heads & ((1ull << lane) - 1));
-        s.begin[at] = v.x * scale;
-        s.end[at] = v.y * scale;
+        s.begin[at] = v.x;
+        s.end[at] = v.y;
       }
       count += __popcll(heads);
       last.x = __shfl(v.x, 63);
@@ -402,19 +441,29 @@ collect_spans(Spans<ROWS> &s, const int2 *spans, int row0, int rows, int group,
 }
 
 // The tiles of this workgroup's piece, in order: rows [begin, end of the tile or of its
-// span).  All of it is the same in every lane and kept in scalar registers.
+// span), the whole list once for each of `rounds` heads.  All of it is the same in every
+// lane and kept in scalar registers.
 template <int ROWS> struct Walk {
   const Spans<ROWS> &s;
-  int left, span, first, begin, end, tile;
-  __device__ __forceinline__ Walk(const Spans<ROWS> &spans, int piece,
-                                  int pieces, int tile_rows)
-      : s(spans), span(0), first(0), begin(0), end(0), tile(tile_rows) {
-    const int count = __builtin_amdgcn_readfirstlane(s.count);
-    const int total =
+  int left, round, count, span, first, begin, end, tile;
+  __device__ __forceinline__ Walk(const Spans<ROWS> &spans, int rounds,
+                                  int piece, int pieces, int tile_rows)
+      : s(spans), round(0), span(0), first(0), begin(0), end(0),
+        tile(tile_rows) {
+    count = __builtin_amdgcn_readfirstlane(s.count);
+    const int once =
         count > 0 ? __builtin_amdgcn_readfirstlane(s.first[count]) : 0;
-    const int at = (int)((int64_t)total * piece / pieces);
-    left = (int)((int64_t)total * (piece + 1) / pieces) - at;
+    const int total = once * rounds;
+    // (the first total % pieces pieces have one tile more)
+    const int share = pieces == 1 ? total : total / pieces;
+    const int more = total - share * pieces;
+    int at = share * piece + min(piece, more);
+    left = share + (piece < more);
     if (left > 0) {
+      if (rounds > 1) {
+        round = at / once;
+        at -= round * once;
+      }
       while (__builtin_amdgcn_readfirstlane(s.first[span + 1]) <= at)
         ++span;
       enter();
@@ -430,7 +479,10 @@ template <int ROWS> struct Walk {
     --left;
     begin += tile;
     if (begin >= end && left > 0) { // (no span is empty)
-      ++span;
+      if (++span == count) {
+        span = 0;
+        ++round;
+      }
       enter();
     }
   }
@@ -451,6 +503,11 @@ struct Place {
     head = b / pieces / tiles;
   }
 };
+
+// Waves per SIMD that the registers are cut to.
+template <typename T, int DP, int RB, int WK> constexpr int waves_wanted() {
+  return WK > 1 && DP > 64 ? 1 : sizeof(T) == 2 && DP <= 64 && RB == 1 && WK == 1 ? 4 : 2;
+}
 
 // Rows of looped tiles per wave and step: the tile's 16-byte pieces fill the threads.
 template <typename T, int WK> struct Looped {
@@ -513,10 +570,52 @@ template <int RB> struct Members {
   }
 };
 
+// Sums of a wave's columns: blocks of d, blocks of columns.
+template <typename T, int DP, int RB> using Sums = f32x4[Shape<T, DP>::DB][RB];
+
+// acc += (rows of the tile from row0, turned) p.  Where the columns belong to several
+// examples, only those that the tile belongs to: the others' sums stay as they are,
+// whatever the tile holds.
+template <typename T, int DP, int RB>
+__device__ __forceinline__ void add_product(Sums<T, DP, RB> &acc,
+                                            const char *tile, int row0,
+                                            const u32x4 (&p)[RB],
+                                            const Members<RB> &members) {
+  using S = Shape<T, DP>;
+  if (members.mixed) {
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db) {
+      const u32x4 a = turned_operand<T, DP>(tile, row0, db);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb) {
+        f32x4 t = acc[db][rb];
+        mma<T>(t, a, p[rb]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          acc[db][rb][r] = members.in[rb] ? t[r] : acc[db][rb][r];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int db = 0; db < S::DB; ++db) {
+      const u32x4 a = turned_operand<T, DP>(tile, row0, db);
+#pragma unroll
+      for (int rb = 0; rb < RB; ++rb)
+        mma<T>(acc[db][rb], a, p[rb]);
+    }
+  }
+}
+
 // Scores in units of log 2 less `base` (per block and row of it), from products.  With
 // a cap, `flat` gets 1 - tanh^2 (in fp32) or a quarter of it: kFlatUp.
 template <typename T>
 constexpr float kFlatUp = std::is_same<T, float>::value ? 1.f : 4.f;
+
+// What cap_scores adds to every score: it wants `base` less this.
+template <typename T>
+__device__ __forceinline__ float under_cap(const AttentionCall &c) {
+  return c.cap > 0.f && !std::is_same<T, float>::value ? c.cap * kLog2e : 0.f;
+}
 
 template <typename T, bool FLAT>
 __device__ __forceinline__ void cap_scores(f32x4 &s, const AttentionCall &c,
@@ -530,10 +629,10 @@ __device__ __forceinline__ void cap_scores(f32x4 &s, const AttentionCall &c,
       if constexpr (FLAT)
         (*flat)[r] = fmaf(-t, t, 1.f);
     } else {
-      // tanh = 1 - 2 w, 1 - tanh^2 = 4 (w - w^2)
+      // tanh = 1 - 2 w (the 1 is in base: under_cap), 1 - tanh^2 = 4 (w - w^2)
       const float w =
           __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * in) + 1.f);
-      s[r] = fmaf(w, -2.f * out, out - base[r]);
+      s[r] = fmaf(w, -2.f * out, -base[r]);
       if constexpr (FLAT)
         (*flat)[r] = fmaf(-w, w, w);
     }
@@ -551,22 +650,34 @@ __device__ __forceinline__ float far_by(const float (&p)[3], float x, float y,
   return __builtin_amdgcn_sqrtf(fmaf(e, e, fmaf(b, b, a * a)));
 }
 
-// Positions of rows [begin, end) to LDS, axis by axis (the third of two stays as it is:
-// cleared).
+// Numbers of rows [begin, end) to LDS, `stride` apart in memory.
+template <int KT>
+__device__ __forceinline__ void request_numbers(const float *from, int stride,
+                                                int begin, int end,
+                                                float (&lds)[KT]) {
+  const int lane = threadIdx.x & 63;
+  const int row0 = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64;
+  if (row0 >= KT || (KT < 64 && lane >= KT))
+    return;
+  const float *base = from + (int64_t)(begin + row0) * stride;
+  const uint32_t to = lds_address(&lds[row0]);
+  if (begin + KT <= end)
+    request4(base, (uint32_t)(lane * stride) * 4u, to);
+  else
+    request4(begin + row0 + lane < end ? (const void *)(base + lane * stride)
+                                       : (const void *)kZeros,
+             to);
+}
+// Positions, axis by axis (the third of two stays as it is: cleared).
 template <int KT>
 __device__ __forceinline__ void request_positions(const float *pos, int begin,
                                                   int end, int axes,
                                                   float (*lds)[KT]) {
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (wave * 64 < KT) {
-    const int row = begin + wave * 64 + lane;
-    for (int a = 0; a < axes; ++a)
-      if (KT >= 64 || lane < KT)
-        request4(row < end ? (const void *)(pos + (int64_t)row * axes + a)
-                           : (const void *)kZeros,
-                 lds_address(&lds[a][wave * 64]));
-  }
+  request_numbers<KT>(pos, axes, begin, end, lds[0]);
+  if (axes > 1)
+    request_numbers<KT>(pos + 1, axes, begin, end, lds[1]);
+  if (axes > 2)
+    request_numbers<KT>(pos + 2, axes, begin, end, lds[2]);
 }
 
 // The four looped rows of a block that a lane has scores of: `at`, at + 1, ...
@@ -611,7 +722,7 @@ __device__ __forceinline__ void take_distance(f32x4 (&s)[RB][NB],
 // Rows of a wave's columns: RB blocks of 16.  WK waves share the same columns and
 // divide every tile among them (few rows); the others own columns of their own.
 template <typename T, int DP, int RB, int WK>
-__global__ __launch_bounds__(kThreads, 2) void
+__global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void
 attention_forward_kernel(AttentionCall c) {
   using S = Shape<T, DP>;
   constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
@@ -657,12 +768,12 @@ attention_forward_kernel(AttentionCall c) {
   }
 
   const Requests<T, DP, KT> request_k(c.k, c.d), request_v(c.v, c.d);
-  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
+  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, KT);
   // Two buffers: while a tile is worked on, the next one is on its way.
   auto request = [&](int begin, int end, int buffer) {
     char *tile = lds_tiles + buffer * 2 * TILE;
-    request_k(begin, end, 1, place.head, tile);
-    request_v(begin, end, 1, place.head, tile + TILE);
+    request_k(begin, end, place.head, tile);
+    request_v(begin, end, place.head, tile + TILE);
     if (c.slope)
       request_positions<KT>(c.pos_k, begin, end, c.axes, lds_pos[buffer]);
   };
@@ -671,7 +782,7 @@ attention_forward_kernel(AttentionCall c) {
   if (c.d < DP)
     clear_lds<4 * TILE>(lds_tiles);
 
-  Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  Walk<ROWS> walk(spans, 1, place.piece, c.splits, KT);
   int buffer = 0;
   Members<RB> members;
   if (walk.there())
@@ -713,7 +824,8 @@ attention_forward_kernel(AttentionCall c) {
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-          cap_scores<T, false>(s[rb][kb], c, all4(m[rb]), nullptr);
+          cap_scores<T, false>(s[rb][kb], c, all4(m[rb] - under_cap<T>(c)),
+                               nullptr);
     } else {
       const float in = c.scale * kLog2e;
 #pragma unroll
@@ -792,22 +904,7 @@ attention_forward_kernel(AttentionCall c) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
         p[rb] = block_operand<T>(&s[rb][f * S::FB]);
-#pragma unroll
-      for (int db = 0; db < S::DB; ++db) {
-        const u32x4 a = turned_operand<T, DP>(lds_v, f * S::KF, db);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          if (mixed) {
-            f32x4 t = acc[db][rb];
-            mma<T>(t, a, p[rb]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              acc[db][rb][r] = in[rb] ? t[r] : acc[db][rb][r];
-          } else {
-            mma<T>(acc[db][rb], a, p[rb]);
-          }
-        }
-      }
+      add_product<T, DP, RB>(acc, lds_v, f * S::KF, p, members);
     }
   }
 
@@ -888,8 +985,11 @@ attention_forward_kernel(AttentionCall c) {
         if (WK > 1 && db % kWaves != wave)
           continue;
         const int e = db * 16 + g * 4;
-        store4<T>(static_cast<T *>(c.out) + at * c.d + e, acc[db][rb] * inv,
-                  c.d - e, vec);
+        const f32x4 v = acc[db][rb] * inv;
+        store4<T>(static_cast<T *>(c.out) + at * c.d + e, v, c.d - e, vec);
+        if (c.rest)
+          store4<T>(static_cast<T *>(c.rest) + at * c.d + e, rest4<T>(v),
+                    c.d - e, vec);
       }
       if (first && c.lse)
         c.lse[(int64_t)col[rb].head * c.nq + col[rb].row] =
@@ -932,9 +1032,6 @@ template <typename T> struct Range {
 // number of rows).
 template <typename T>
 constexpr float kWeightUp = std::is_same<T, _Float16>::value ? 0x1p14f : 1.f;
-
-// Sums of a wave's columns: blocks of d, blocks of columns.
-template <typename T, int DP, int RB> using Sums = f32x4[Shape<T, DP>::DB][RB];
 
 // WK waves' sums of the same 16 columns, in the order of the waves: afterwards wave w
 // holds blocks w, w + 4, ... of d.
@@ -982,10 +1079,10 @@ store_columns(const Sums<T, DP, RB> &acc, int rb, void *out, float *part,
   }
 }
 
-// dq of the rows that a workgroup owns, looping over keys; writes delta for the kernel
-// of dk and dv.
+// dq of the rows that a workgroup owns, looping over keys; writes what the kernel of dk
+// and dv takes of a row.
 template <typename T, int DP, int RB, int WK>
-__global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall c) {
+__global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void attention_dq_kernel(AttentionCall c) {
   using S = Shape<T, DP>;
   constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
   constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
@@ -1012,11 +1109,13 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
   for (int rb = 0; rb < RB; ++rb) {
     col[rb] = query_column(c, row0 + (wq * RB + rb) * 16 + i, group,
                            place.head * group);
-    HeadRows out;
+    HeadRows out, rest;
     out.data = c.out_in;
     out.row = (int64_t)c.hq * c.d;
     out.head = c.d;
     out.vec = c.d * S::SZ % 16 == 0;
+    rest = out;
+    rest.data = c.rest;
     float sum = 0.f;
 #pragma unroll
     for (int ks = 0; ks < S::KS; ++ks) {
@@ -1035,6 +1134,14 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
 #pragma unroll
         for (int e = 0; e < S::PER; ++e)
           sum = fmaf(to_float(a[e]), to_float(b[e]), sum);
+        if (c.rest) {
+          const u32x4 l =
+              load_piece<T, DP>(rest, col[rb].row, col[rb].head, piece, c.d);
+          __builtin_memcpy(a, &l, 16);
+#pragma unroll
+          for (int e = 0; e < S::PER; ++e)
+            sum = fmaf(to_float(a[e]), to_float(b[e]), sum);
+        }
       }
     }
     delta[rb] = across_groups_sum(sum);
@@ -1042,8 +1149,11 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
     if (col[rb].valid) {
       const int64_t at = (int64_t)col[rb].head * c.nq + col[rb].row;
       lse[rb] = c.lse[at];
-      if (place.piece == 0 && g == 0 && (WK == 1 || wave == 0))
-        c.delta[at] = delta[rb];
+      if (place.piece == 0 && g == 0 && (WK == 1 || wave == 0)) {
+        // as the kernel of dk and dv adds them
+        c.minus_delta[at] = -delta[rb];
+        c.base[at] = lse[rb] - under_cap<T>(c);
+      }
     }
 #pragma unroll
     for (int db = 0; db < S::DB; ++db)
@@ -1051,12 +1161,15 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
   }
 
   const Requests<T, DP, KT> request_k(c.k, c.d), request_v(c.v, c.d);
-  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, 1, KT);
+  if (c.slope && blockIdx.x == 0)
+    for (int h = threadIdx.x; h < c.hq; h += kThreads)
+      c.minus_slope[h] = c.slope[h] * -kLog2e;
+  collect_spans<ROWS>(spans, c.spans_q, row0, rows, group, c.nk, KT);
   // Two buffers: while a tile is worked on, the next one is on its way.
   auto request = [&](int begin, int end, int buffer) {
     char *tile = lds_tiles + buffer * 2 * TILE;
-    request_k(begin, end, 1, place.head, tile);
-    request_v(begin, end, 1, place.head, tile + TILE);
+    request_k(begin, end, place.head, tile);
+    request_v(begin, end, place.head, tile + TILE);
     if (c.slope)
       request_positions<KT>(c.pos_k, begin, end, c.axes, lds_pos[buffer]);
   };
@@ -1065,7 +1178,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
   if (c.d < DP)
     clear_lds<4 * TILE>(lds_tiles);
 
-  Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  Walk<ROWS> walk(spans, 1, place.piece, c.splits, KT);
   int buffer = 0;
   Members<RB> members;
   if (walk.there())
@@ -1113,7 +1226,8 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int b = 0; b < S::FB; ++b)
-            cap_scores<T, true>(s[rb][b], c, all4(lse[rb]), &flat[rb][b]);
+            cap_scores<T, true>(s[rb][b], c, all4(lse[rb] - under_cap<T>(c)),
+                                &flat[rb][b]);
       } else {
         const float in = c.scale * kLog2e;
 #pragma unroll
@@ -1183,22 +1297,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
         p[rb] = block_operand<T>(ds[rb]);
-#pragma unroll
-      for (int db = 0; db < S::DB; ++db) {
-        const u32x4 a = turned_operand<T, DP>(lds_k, f * S::KF, db);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          if (mixed) {
-            f32x4 t = acc[db][rb];
-            mma<T>(t, a, p[rb]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              acc[db][rb][r] = in[rb] ? t[r] : acc[db][rb][r];
-          } else {
-            mma<T>(acc[db][rb], a, p[rb]);
-          }
-        }
-      }
+      add_product<T, DP, RB>(acc, lds_k, f * S::KF, p, members);
     }
   }
 
@@ -1227,7 +1326,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_dq_kernel(AttentionCall
 
 // dk and dv of the keys that a workgroup owns, looping over (query, head) rows.
 template <typename T, int DP, int RB, int WK>
-__global__ __launch_bounds__(kThreads, 2) void
+__global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void
 attention_dkv_kernel(AttentionCall c) {
   using S = Shape<T, DP>;
   constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
@@ -1235,7 +1334,8 @@ attention_dkv_kernel(AttentionCall c) {
   constexpr int KB = KW / 16;
   constexpr int TILE = KT * S::BYTES;
   __shared__ __attribute__((aligned(16))) char lds_tiles[4 * TILE];
-  // per looped row: position, slope, lse, delta
+  // per looped row: position, -slope (times log2 e), what its scores are relative to
+  // (cap_scores), -delta
   __shared__ __attribute__((aligned(16))) float lds_row[2][6][KT];
   __shared__ Spans<ROWS> spans;
 
@@ -1258,8 +1358,6 @@ attention_dkv_kernel(AttentionCall c) {
     if (col[rb].valid) {
       col[rb].row = row;
       col[rb].span = c.spans_k ? c.spans_k[row] : make_int2(0, c.nq);
-      col[rb].span.x *= group;
-      col[rb].span.y *= group;
       if (c.slope)
         load_position(col[rb].p, c.pos_k, row, c.axes);
     }
@@ -1277,28 +1375,20 @@ attention_dkv_kernel(AttentionCall c) {
   }
 
   const Requests<T, DP, KT> request_q(c.q, c.d), request_do(c.dout, c.d);
-  collect_spans<ROWS>(spans, c.spans_k, row0, c.nk, 1, c.nq, group, KT);
+  collect_spans<ROWS>(spans, c.spans_k, row0, c.nk, 1, c.nq, KT);
   // Two buffers: while a tile is worked on, the next one is on its way.
-  auto request = [&](int begin, int end, int buffer) {
+  auto request = [&](int begin, int end, int round, int buffer) {
     char *tile = lds_tiles + buffer * 2 * TILE;
-    request_q(begin, end, group, head0, tile);
-    request_do(begin, end, group, head0, tile + TILE);
-    const int w = __builtin_amdgcn_readfirstlane(wave);
-    const int row = begin + w * 64 + lane;
-    if (w * 64 < KT && (KT >= 64 || lane < KT)) {
-      const int query = row / group, head = head0 + row - query * group;
-      auto one = [&](int what, const float *from) {
-        request4(row < end ? (const void *)from : (const void *)kZeros,
-                 lds_address(&lds_row[buffer][what][w * 64]));
-      };
-      const int64_t at = (int64_t)head * c.nq + query;
-      one(4, c.lse + at);
-      one(5, c.delta + at);
-      if (c.slope) {
-        for (int a = 0; a < c.axes; ++a)
-          one(a, c.pos_q + (int64_t)query * c.axes + a);
-        one(3, c.slope + head);
-      }
+    const int head = head0 + round;
+    request_q(begin, end, head, tile);
+    request_do(begin, end, head, tile + TILE);
+    auto &rows = lds_row[buffer];
+    request_numbers<KT>(c.base + (int64_t)head * c.nq, 1, begin, end, rows[4]);
+    request_numbers<KT>(c.minus_delta + (int64_t)head * c.nq, 1, begin, end,
+                        rows[5]);
+    if (c.slope) {
+      request_positions<KT>(c.pos_q, begin, end, c.axes, rows);
+      request_numbers<KT>(c.minus_slope + head, 0, begin, end, rows[3]);
     }
   };
   if (c.axes == 2)
@@ -1306,18 +1396,18 @@ attention_dkv_kernel(AttentionCall c) {
   if (c.d < DP)
     clear_lds<4 * TILE>(lds_tiles);
 
-  Walk<ROWS> walk(spans, place.piece, c.splits, KT);
+  Walk<ROWS> walk(spans, group, place.piece, c.splits, KT);
   int buffer = 0;
   Members<RB> members;
   if (walk.there())
-    request(walk.begin, walk.end, 0);
+    request(walk.begin, walk.end, walk.round, 0);
   for (; walk.there(); buffer ^= 1) {
     const int begin = walk.begin, end = walk.end;
     members.of(walk.span, walk.first, end, col);
     arrive();
     walk.next();
     if (walk.there())
-      request(walk.begin, walk.end, buffer ^ 1);
+      request(walk.begin, walk.end, walk.round, buffer ^ 1);
     const char *lds_q = lds_tiles + buffer * 2 * TILE + part * S::BYTES;
     const char *lds_do = lds_q + TILE;
 
@@ -1335,12 +1425,12 @@ attention_dkv_kernel(AttentionCall c) {
 #pragma unroll
       for (int b = 0; b < S::FB; ++b) {
         lse[b] = *reinterpret_cast<const f32x4 *>(&rows[4][at + b * 16]);
-        const f32x4 delta =
+        const f32x4 minus_delta =
             *reinterpret_cast<const f32x4 *>(&rows[5][at + b * 16]);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
           pr[rb][b] = f32x4{0, 0, 0, 0};
-          ds[rb][b] = -delta;
+          ds[rb][b] = minus_delta;
         }
 #pragma unroll
         for (int ks = 0; ks < S::KS; ++ks) {
@@ -1373,8 +1463,7 @@ attention_dkv_kernel(AttentionCall c) {
 #pragma unroll
         for (int b = 0; b < S::FB; ++b) {
           const f32x4 slope =
-              *reinterpret_cast<const f32x4 *>(&rows[3][at + b * 16]) *
-              -kLog2e;
+              *reinterpret_cast<const f32x4 *>(&rows[3][at + b * 16]);
           const f32x4 x =
               *reinterpret_cast<const f32x4 *>(&rows[0][at + b * 16]);
           if (c.axes == 1) {
@@ -1466,27 +1555,8 @@ attention_dkv_kernel(AttentionCall c) {
         p[rb] = block_operand<T>(pr[rb]);
         x[rb] = block_operand<T>(ds[rb]);
       }
-#pragma unroll
-      for (int db = 0; db < S::DB; ++db) {
-        const u32x4 a = turned_operand<T, DP>(lds_do, f * S::KF, db);
-        const u32x4 b = turned_operand<T, DP>(lds_q, f * S::KF, db);
-#pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-          if (mixed) {
-            f32x4 t = acc_v[db][rb], u = acc_k[db][rb];
-            mma<T>(t, a, p[rb]);
-            mma<T>(u, b, x[rb]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              acc_v[db][rb][r] = in[rb] ? t[r] : acc_v[db][rb][r];
-              acc_k[db][rb][r] = in[rb] ? u[r] : acc_k[db][rb][r];
-            }
-          } else {
-            mma<T>(acc_v[db][rb], a, p[rb]);
-            mma<T>(acc_k[db][rb], b, x[rb]);
-          }
-        }
-      }
+      add_product<T, DP, RB>(acc_v, lds_do, f * S::KF, p, members);
+      add_product<T, DP, RB>(acc_k, lds_q, f * S::KF, x, members);
     }
   }
 
@@ -1535,11 +1605,11 @@ hipError_t launch(const AttentionCall &c, int pass, int rows,
   else                                                                         \
     kernel<T, DP, most / 64, 1><<<g, b, 0, stream>>>(c)
   if (pass == 0) {
-    PCA_LAUNCH(attention_forward_kernel, most_rows(0, sizeof(T), DP));
+    PCA_LAUNCH(attention_forward_kernel, most_rows(0, DP));
   } else if (pass == 1) {
-    PCA_LAUNCH(attention_dq_kernel, most_rows(1, sizeof(T), DP));
+    PCA_LAUNCH(attention_dq_kernel, most_rows(1, DP));
   } else {
-    PCA_LAUNCH(attention_dkv_kernel, most_rows(2, sizeof(T), DP));
+    PCA_LAUNCH(attention_dkv_kernel, most_rows(2, DP));
   }
 #undef PCA_LAUNCH
   return hipGetLastError();

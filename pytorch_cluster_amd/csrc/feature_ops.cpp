@@ -114,7 +114,7 @@ struct Attention {
   Tensor workspace(bool backward) const {
     const size_t bytes = pca_attention_workspace_bytes(
         q.size(0), k.size(0), (int32_t)q.size(1), (int32_t)k.size(1),
-        (int32_t)q.size(2), dtype_code(q), backward);
+        (int32_t)q.size(2), backward);
     TORCH_CHECK(bytes > 0, "attention: problem size not supported");
     return scratch(bytes, q);
   }
@@ -135,16 +135,20 @@ bool same_rows(const Tensor &a, const Tensor &b) {
   return a.data_ptr() == b.data_ptr() && a.numel() == b.numel();
 }
 
-Tensor attention_forward(const Attention &a, Tensor *lse) {
+// lse and rest: for the backward pass, or NULL.
+Tensor attention_forward(const Attention &a, Tensor *lse, Tensor *rest) {
   auto out = at::empty(a.q.sizes(), a.q.options().memory_format(
                                         at::MemoryFormat::Contiguous));
   if (lse)
     *lse = at::empty({a.q.size(1), a.q.size(0)},
                      a.q.options().dtype(at::kFloat));
+  if (rest && a.q.scalar_type() != at::kFloat)
+    *rest = at::empty_like(out);
   const auto workspace = a.workspace(false);
   const auto args = a.args();
   check_status(pca_attention_forward(
       &args, const_cast<void *>(data_or_null(out)),
+      rest ? const_cast<void *>(data_or_null(*rest)) : nullptr,
       lse ? static_cast<float *>(const_cast<void *>(data_or_null(*lse)))
           : nullptr,
       workspace.data_ptr(), (size_t)workspace.numel(), current_stream(a.q)));
@@ -169,10 +173,10 @@ struct AttentionFunction
     a.cap = cap;
     if (ids_q.defined())
       a.spans_q = spans_of(ids_q, ids_k);
-    Tensor lse;
-    auto out = attention_forward(a, &lse);
+    Tensor lse, rest;
+    auto out = attention_forward(a, &lse, &rest);
     ctx->save_for_backward({q, k, v, out, lse, ids_q, ids_k, a.pos_q, a.pos_k,
-                            a.slope, a.spans_q});
+                            a.slope, a.spans_q, rest});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["cap"] = cap;
     return out;
@@ -205,7 +209,7 @@ struct AttentionFunction
     const auto workspace = a.workspace(true);
     const auto args = a.args();
     check_status(pca_attention_backward(
-        &args, data_or_null(out),
+        &args, data_or_null(out), data_or_null(saved[11]),
         static_cast<const float *>(data_or_null(lse)), data_or_null(dout),
         dout.stride(0), dout.stride(1), const_cast<void *>(data_or_null(dq)),
         const_cast<void *>(data_or_null(dk)),
@@ -307,7 +311,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v,
   a.cap = cap;
   if (ids_q.defined())
     a.spans_q = spans_of(ids_q, ids_k);
-  return attention_forward(a, nullptr);
+  return attention_forward(a, nullptr, nullptr);
 }
 
 // ---- norm_rotate ------------------------------------------------------------------

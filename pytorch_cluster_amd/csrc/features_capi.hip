@@ -197,31 +197,30 @@ int pca_spans(const int64_t *ids_a, int64_t na, const int64_t *ids_b,
 }
 
 size_t pca_attention_workspace_bytes(int64_t nq, int64_t nk, int32_t hq,
-                                     int32_t hk, int32_t d, int32_t dtype,
-                                     int backward) {
-  if (!attention_sizes_ok(nq, nk, hq, hk, d) || !type_ok(dtype))
+                                     int32_t hk, int32_t d, int backward) {
+  if (!attention_sizes_ok(nq, nk, hq, hk, d))
     return 0;
-  return pca::attention_workspace_bytes(backward ? 1 : 0, nq, nk, hq, hk, dtype,
-                                        d);
+  return pca::attention_workspace_bytes(backward ? 1 : 0, nq, nk, hq, hk, d);
 }
 
-int pca_attention_forward(const pca_attention_args *args, void *out, float *lse,
-                          void *workspace, size_t workspace_bytes,
+int pca_attention_forward(const pca_attention_args *args, void *out, void *rest,
+                          float *lse, void *workspace, size_t workspace_bytes,
                           void *stream) {
   pca::AttentionCall c;
   int rc = attention_call(args, c);
   if (rc != PCA_OK)
     return rc;
-  if (args->nq > 0 && (out == nullptr || !on16(out)))
+  if (args->nq > 0 && (out == nullptr || !on16(out) || !on16(rest)))
     return pca::fail(PCA_ERR_INVALID_ARGUMENT,
-                     "attention: out has to start on 16 bytes");
+                     "attention: out and rest have to start on 16 bytes");
   rc = no_workspace("attention",
                     pca::attention_workspace_bytes(0, c.nq, c.nk, c.hq, c.hk,
-                                                   args->dtype, c.d),
+                                                   c.d),
                     workspace, workspace_bytes);
   if (rc != PCA_OK)
     return rc;
   c.out = out;
+  c.rest = rest;
   c.lse = lse;
   return launched(pca::attention_forward(c, args->dtype, workspace,
                                          static_cast<hipStream_t>(stream)),
@@ -229,10 +228,10 @@ int pca_attention_forward(const pca_attention_args *args, void *out, float *lse,
 }
 
 int pca_attention_backward(const pca_attention_args *args, const void *out,
-                           const float *lse, const void *dout, int64_t dout_row,
-                           int64_t dout_head, void *dq, void *dk, void *dv,
-                           void *workspace, size_t workspace_bytes,
-                           void *stream) {
+                           const void *rest, const float *lse, const void *dout,
+                           int64_t dout_row, int64_t dout_head, void *dq,
+                           void *dk, void *dv, void *workspace,
+                           size_t workspace_bytes, void *stream) {
   pca::AttentionCall c;
   int rc = attention_call(args, c);
   if (rc != PCA_OK)
@@ -242,7 +241,7 @@ int pca_attention_backward(const pca_attention_args *args, const void *out,
       (c.nk > 0 && (dk == nullptr || dv == nullptr)))
     return pca::fail(PCA_ERR_INVALID_ARGUMENT,
                      "attention backward: a tensor is NULL");
-  if (!on16(out) || !on16(dq) || !on16(dk) || !on16(dv))
+  if (!on16(out) || !on16(rest) || !on16(dq) || !on16(dk) || !on16(dv))
     return pca::fail(PCA_ERR_INVALID_ARGUMENT,
                      "attention backward: dense tensors have to start on 16 "
                      "bytes");
@@ -252,11 +251,12 @@ int pca_attention_backward(const pca_attention_args *args, const void *out,
                      "attention backward: spans of one side only");
   rc = no_workspace("attention backward",
                     pca::attention_workspace_bytes(1, c.nq, c.nk, c.hq, c.hk,
-                                                   args->dtype, c.d),
+                                                   c.d),
                     workspace, workspace_bytes);
   if (rc != PCA_OK)
     return rc;
   c.out_in = out;
+  c.rest = const_cast<void *>(rest);
   c.lse = const_cast<float *>(lse);
   c.dout = head_rows(dout, dout_row, dout_head, c.d, args->dtype);
   c.dq = dq;

@@ -127,9 +127,9 @@ def test_c_abi_checks_before_any_launch():
         a = _native.AttentionArgs.from_buffer_copy(args)
         for name, value in change.items():
             setattr(a, name, value)
-        return lib.pca_attention_forward(ctypes.byref(a), out, None, ws, size,
-                                         None)
-    assert lib.pca_attention_forward(None, at, None, at, 1 << 20, None) == -1
+        return lib.pca_attention_forward(ctypes.byref(a), out, None, None, ws,
+                                         size, None)
+    assert lib.pca_attention_forward(None, at, None, None, at, 1 << 20, None) == -1
     assert forward(dtype=1) == -5
     assert forward(d=129) == -5
     assert b"up to 128" in lib.pca_last_error()
@@ -147,17 +147,16 @@ def test_c_abi_checks_before_any_launch():
     assert forward(size=16) == -3
     assert forward(ws=at + 8) == -3
     assert forward(ws=None) == -3
-    assert lib.pca_attention_workspace_bytes(10, 10, 4, 3, 64, 0, 0) == 0
-    assert lib.pca_attention_workspace_bytes(10, 10, 4, 2, 64, 0, 1) > 0
-    assert lib.pca_attention_workspace_bytes(10, 10, 4, 2, 64, 1, 1) == 0
+    assert lib.pca_attention_workspace_bytes(10, 10, 4, 3, 64, 0) == 0
+    assert lib.pca_attention_workspace_bytes(10, 10, 4, 2, 64, 1) > 0
 
     def backward(dq=at, lse=at, **change):
         a = _native.AttentionArgs.from_buffer_copy(args)
         for name, value in change.items():
             setattr(a, name, value)
         return lib.pca_attention_backward(
-            ctypes.byref(a), at, lse, at, 256, 64, dq, at, at, at, 1 << 30,
-            None)
+            ctypes.byref(a), at, None, lse, at, 256, 64, dq, at, at, at,
+            1 << 30, None)
     assert backward(lse=None) == -1
     assert backward(dq=None) == -1
     assert backward(dq=at + 2) == -1
