@@ -215,8 +215,11 @@ join_sum_kernel(const float *part, int pieces, int64_t stride, int64_t count,
 
 AttentionLauncher launcher(int dtype, int d) {
 #define PCA_BY_WIDTH(type)                                                     \
-  (d <= 32 ? attention_##type##_d32                                            \
-           : d <= 64 ? attention_##type##_d64 : attention_##type##_d128)
+  (d <= 32   ? attention_##type##_d32                                          \
+   : d <= 48 ? attention_##type##_d48                                          \
+   : d <= 64 ? attention_##type##_d64                                          \
+   : d <= 96 ? attention_##type##_d96                                          \
+             : attention_##type##_d128)
   return dtype == 0 ? PCA_BY_WIDTH(f32)
                     : dtype == 2 ? PCA_BY_WIDTH(f16) : PCA_BY_WIDTH(bf16);
 #undef PCA_BY_WIDTH

@@ -54,14 +54,18 @@ struct AttentionPlan {
   int splits = 1;
 };
 
-// One per element type (0 fp32, 2 fp16, 3 bf16: pca_dtype) and width of a head (32,
-// 64, 128): attention_<type>_d<width>.hip.  `pass`: 0 forward, 1 dq, 2 dk and dv.
+// One per element type (0 fp32, 2 fp16, 3 bf16: pca_dtype) and width of a head:
+// attention_<type>_d<width>.hip.  `pass`: 0 forward, 1 dq, 2 dk and dv.
 typedef hipError_t (*AttentionLauncher)(const AttentionCall &, int pass,
                                         int rows, hipStream_t);
 #define PCA_ATTENTION_DECLARE(type)                                            \
   hipError_t attention_##type##_d32(const AttentionCall &, int, int,           \
                                     hipStream_t);                              \
+  hipError_t attention_##type##_d48(const AttentionCall &, int, int,           \
+                                    hipStream_t);                              \
   hipError_t attention_##type##_d64(const AttentionCall &, int, int,           \
+                                    hipStream_t);                              \
+  hipError_t attention_##type##_d96(const AttentionCall &, int, int,           \
                                     hipStream_t);                              \
   hipError_t attention_##type##_d128(const AttentionCall &, int, int,          \
                                      hipStream_t)

@@ -3,7 +3,7 @@
 
 namespace pca {
 hipError_t attention_bf16_d128(const AttentionCall &c, int pass, int rows,
-                          hipStream_t stream) {
+                               hipStream_t stream) {
   return attn::launch<__bf16, 128>(c, pass, rows, stream);
 }
 } // namespace pca

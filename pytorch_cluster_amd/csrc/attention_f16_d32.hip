@@ -3,7 +3,7 @@
 
 namespace pca {
 hipError_t attention_f16_d32(const AttentionCall &c, int pass, int rows,
-                          hipStream_t stream) {
+                             hipStream_t stream) {
   return attn::launch<_Float16, 32>(c, pass, rows, stream);
 }
 } // namespace pca

@@ -1,0 +1,9 @@
+// Attention kernels: f16, heads of up to 48.
+#include "attention_impl.hpp"
+
+namespace pca {
+hipError_t attention_f16_d48(const AttentionCall &c, int pass, int rows,
+                             hipStream_t stream) {
+  return attn::launch<_Float16, 48>(c, pass, rows, stream);
+}
+} // namespace pca

@@ -3,7 +3,7 @@
 
 namespace pca {
 hipError_t attention_f32_d32(const AttentionCall &c, int pass, int rows,
-                          hipStream_t stream) {
+                             hipStream_t stream) {
   return attn::launch<float, 32>(c, pass, rows, stream);
 }
 } // namespace pca

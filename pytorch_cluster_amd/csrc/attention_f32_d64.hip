@@ -3,7 +3,7 @@
 
 namespace pca {
 hipError_t attention_f32_d64(const AttentionCall &c, int pass, int rows,
-                          hipStream_t stream) {
+                             hipStream_t stream) {
   return attn::launch<float, 64>(c, pass, rows, stream);
 }
 } // namespace pca

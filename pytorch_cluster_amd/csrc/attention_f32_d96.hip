@@ -1,0 +1,9 @@
+// Attention kernels: f32, heads of up to 96.
+#include "attention_impl.hpp"
+
+namespace pca {
+hipError_t attention_f32_d96(const AttentionCall &c, int pass, int rows,
+                             hipStream_t stream) {
+  return attn::launch<float, 96>(c, pass, rows, stream);
+}
+} // namespace pca

@@ -80,14 +80,16 @@ __device__ __forceinline__ void mma(f32x4 &acc, u32x4 a, u32x4 b) {
   }
 }
 
-// Sizes that follow from the element type and the (padded) width of a head.
+// Sizes that follow from the element type and the width of a head that a kernel is built
+// for: what is computed goes by it, what lies in LDS by the next power of two.
 template <typename T, int DP> struct Shape {
   static constexpr int SZ = sizeof(T);
   static constexpr int PER = 16 / SZ;          // elements of 16 bytes
-  static constexpr int CH = DP / PER;          // 16-byte pieces of a row
-  static constexpr int KS = CH / 4;            // steps of a product over d
+  static constexpr int LDS = DP <= 32 ? 32 : DP <= 64 ? 64 : 128;
+  static constexpr int CH = LDS / PER;         // 16-byte pieces of a row
+  static constexpr int KS = (DP * SZ + 63) / 64; // steps of a product over d
   static constexpr int DB = DP / 16;           // 16-wide blocks over d
-  static constexpr int BYTES = DP * SZ;        // of a row in LDS
+  static constexpr int BYTES = LDS * SZ;       // of a row in LDS
   static constexpr int KF = SZ == 2 ? 32 : 16; // rows of a step over rows
   static constexpr int FB = KF / 16;           // ... in blocks
   // A tile's rows lie in LDS one after the other, as the loads that bypass the
@@ -779,7 +781,7 @@ attention_forward_kernel(AttentionCall c) {
   };
   if (c.axes == 2)
     clear_lds<sizeof(lds_pos)>(reinterpret_cast<char *>(lds_pos));
-  if (c.d < DP)
+  if (c.d < S::LDS)
     clear_lds<4 * TILE>(lds_tiles);
 
   Walk<ROWS> walk(spans, 1, place.piece, c.splits, KT);
@@ -1175,7 +1177,7 @@ __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void att
   };
   if (c.axes == 2)
     clear_lds<sizeof(lds_pos)>(reinterpret_cast<char *>(lds_pos));
-  if (c.d < DP)
+  if (c.d < S::LDS)
     clear_lds<4 * TILE>(lds_tiles);
 
   Walk<ROWS> walk(spans, 1, place.piece, c.splits, KT);
@@ -1393,7 +1395,7 @@ attention_dkv_kernel(AttentionCall c) {
   };
   if (c.axes == 2)
     clear_lds<sizeof(lds_row)>(reinterpret_cast<char *>(lds_row));
-  if (c.d < DP)
+  if (c.d < S::LDS)
     clear_lds<4 * TILE>(lds_tiles);
 
   Walk<ROWS> walk(spans, group, place.piece, c.splits, KT);

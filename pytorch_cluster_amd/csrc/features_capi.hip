@@ -11,7 +11,9 @@
 
 namespace {
 
-constexpr int64_t kMost = 2147483646; // rows of a side, entries
+constexpr int64_t kMost = 2147483646; // rows, entries
+// Rows of attention's sides (times heads of a group): with room for a tile behind them.
+constexpr int64_t kMostOwned = kMost - 1024;
 
 bool type_ok(int dtype) {
   return dtype == PCA_F32 || dtype == PCA_F16 || dtype == PCA_BF16;
@@ -53,8 +55,9 @@ pca::HeadRows head_rows(const void *data, int64_t row, int64_t head, int64_t d,
 
 bool attention_sizes_ok(int64_t nq, int64_t nk, int64_t hq, int64_t hk,
                         int64_t d) {
-  return nq >= 0 && nk >= 0 && nk <= kMost && hk >= 1 && hq >= hk &&
-         hq % hk == 0 && hq <= 65535 && nq <= kMost / (hq / hk) && d >= 1 &&
+  return nq >= 0 && nk >= 0 && nk <= kMostOwned && hk >= 1 && hq >= hk &&
+         hq % hk == 0 && hq <= 65535 && nq <= kMostOwned / (hq / hk) &&
+         d >= 1 &&
          d <= PCA_ATTENTION_MAX_D &&
          // (workgroups of 16 owned rows, numbered by an int)
          (nq / 16 + 1) * hq < kMost && (nk / 16 + 1) * hk < kMost;
@@ -184,7 +187,7 @@ extern "C" {
 
 int pca_spans(const int64_t *ids_a, int64_t na, const int64_t *ids_b,
               int64_t nb, int32_t *spans, void *stream) {
-  if (na < 0 || nb < 0 || na > kMost || nb > kMost ||
+  if (na < 0 || nb < 0 || na > kMostOwned || nb > kMostOwned ||
       (na > 0 && (ids_a == nullptr || spans == nullptr)) ||
       (nb > 0 && ids_b == nullptr) ||
       (reinterpret_cast<uintptr_t>(spans) & 7) != 0)
