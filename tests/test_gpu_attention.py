@@ -258,6 +258,30 @@ def test_views_of_one_tensor(dtype, d):
         assert torch.equal(got[n], want[n]), n
 
 
+@pytest.mark.parametrize("row", [4_000_000, 10_000_008])
+def test_rows_far_apart(row):
+    # offsets beyond 2^31 elements; tiles addressed by 32 bits and, where rows
+    # are too far apart for that, by 64
+    x = inputs(15, 30, 600, 2, 2, 64, torch.bfloat16, axes=1)
+    want = call(x)
+    room = torch.empty(600 * row + 128, dtype=torch.bfloat16, device=DEV)
+    far = dict(x)
+    for n, at in (("k", 0), ("v", row // 2)):
+        far[n] = room[at:].as_strided((600, 2, 64), (row, 64, 1)) \
+            .copy_(x[n])
+    assert far["k"].storage_offset() + 599 * row > 2 ** 31
+    got = call(far)
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+    # the same for the rows that dk and dv loop over
+    want = call(dict(x, q=x["k"], k=x["q"], v=x["q"], dout=x["k"],
+                     pos_q=x["pos_k"], pos_k=x["pos_q"]))
+    got = call(dict(x, q=far["k"], k=x["q"], v=x["q"], dout=far["k"],
+                    pos_q=x["pos_k"], pos_k=x["pos_q"]))
+    for n in want:
+        assert torch.equal(got[n], want[n]), n
+
+
 def test_expanded_gradient():
     x = inputs(8, 30, 40, 2, 2, 32, torch.float32)
     q = x["q"].requires_grad_()

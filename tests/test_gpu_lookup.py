@@ -114,6 +114,29 @@ def test_shapes_types_and_strides_of_the_index():
     assert torch.equal(got["out"], want["out"])
 
 
+def test_tables_beyond_2_to_the_31():
+    # elements of the table, and pieces of 16 bytes of the output
+    rows, width = 18_000_000, 128
+    weight = torch.zeros(rows, width, dtype=torch.float16, device=DEV)
+    g = torch.Generator().manual_seed(8)
+    index = torch.randint(0, rows, (5000,), generator=g)
+    index[:3] = torch.tensor([rows - 1, 0, rows - 1])
+    index = index.to(DEV)
+    weight[index] = torch.randn(5000, width, generator=g).half().to(DEV)
+    weight.requires_grad_()
+    out = pca.lookup(weight, index, 2.0)
+    assert torch.equal(out, weight.detach()[index] * 2)
+    dout = torch.randn(5000, width, generator=g).half().to(DEV)
+    grad, = torch.autograd.grad(out, weight, dout)
+    assert grad.shape == weight.shape
+    few, place = torch.unique(index, return_inverse=True)
+    val, err = lookup64(torch.zeros(len(few), width, dtype=torch.float16,
+                                    device=DEV), place, 2.0, dout)
+    check({"dweight": grad[few]}, val, err)
+    grad[few] = 0
+    assert not grad.any()
+
+
 def test_expanded_gradient():
     weight, index, _ = inputs(5, 100, 600, 12, torch.float32)
     w = weight.requires_grad_()
