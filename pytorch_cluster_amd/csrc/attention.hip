@@ -111,29 +111,39 @@ __device__ __forceinline__ float put_as(int dtype, void *out, int64_t at,
                       : put<__bf16>(out, at, v);
 }
 
+// Pieces in use for row (query, head) of q.  (Sides are cut into pieces where there are
+// few workgroups: rows, and their products with heads, are far below 2^31 here.)
+__device__ __forceinline__ int pieces_of(const AttentionCall &c, int row) {
+  const int query = row / c.hq, head = row - query * c.hq;
+  const int group = c.hq / c.hk, kv = head / group;
+  const int tiles = (c.nq * group + c.rows - 1) / c.rows;
+  return c.pieces[kv * tiles + (query * group + head - kv * group) / c.rows];
+}
+
 // Output rows from the pieces' sums, maxima and sums of weights: 32 lanes take four
 // elements each; where there are many pieces, `shares` groups of lanes divide them and
 // meet in LDS, in their order.
 __global__ __launch_bounds__(256) void
 join_forward_kernel(AttentionCall c, int dtype, int shares) {
   __shared__ float lds_acc[8][128], lds_ml[8][2];
-  const int64_t rows = (int64_t)c.nq * c.hq;
+  const int rows = c.nq * c.hq;
   const int grp = threadIdx.x / 32, share = grp % shares;
-  const int64_t row = (int64_t)blockIdx.x * (8 / shares) + grp / shares;
-  const bool there = row < rows;
+  const int row = blockIdx.x * (8 / shares) + grp / shares;
   const int e0 = (threadIdx.x & 31) * 4;
+  const int pieces = row < rows ? pieces_of(c, row) : 1;
+  const bool there = pieces > 1;
   float top = -__builtin_inff(), sum = 0.f;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   if (there) {
 #pragma unroll 8
-    for (int s = share; s < c.splits; s += shares)
-      top = fmaxf(top, c.part_ml[(s * rows + row) * 2]);
+    for (int s = share; s < pieces; s += shares)
+      top = fmaxf(top, c.part_ml[((int64_t)s * rows + row) * 2]);
 #pragma unroll 4
-    for (int s = share; s < c.splits; s += shares) {
-      const float m = c.part_ml[(s * rows + row) * 2];
-      const float l = c.part_ml[(s * rows + row) * 2 + 1];
+    for (int s = share; s < pieces; s += shares) {
+      const float m = c.part_ml[((int64_t)s * rows + row) * 2];
+      const float l = c.part_ml[((int64_t)s * rows + row) * 2 + 1];
       float v[4] = {0.f, 0.f, 0.f, 0.f};
-      const float *from = c.part + (s * rows + row) * c.d + e0;
+      const float *from = c.part + ((int64_t)s * rows + row) * c.d + e0;
       if (c.d % 4 == 0) {
         if (e0 < c.d)
           __builtin_memcpy(v, __builtin_assume_aligned(from, 16), 16);
@@ -183,34 +193,60 @@ join_forward_kernel(AttentionCall c, int dtype, int shares) {
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (e0 + e < c.d) {
-      const int64_t at = row * c.d + e0 + e;
+      const int64_t at = (int64_t)row * c.d + e0 + e;
       const float left = put_as(dtype, c.out, at, acc[e] * inv);
       if (c.rest)
         put_as(dtype, c.rest, at, left);
     }
   if (e0 == 0 && c.lse) {
-    const int64_t query = row / c.hq, head = row % c.hq;
-    c.lse[head * c.nq + query] =
+    const int query = row / c.hq, head = row % c.hq;
+    c.lse[(int64_t)head * c.nq + query] =
         sum == 0.f ? __builtin_inff() : top + __builtin_amdgcn_logf(sum);
   }
 }
 
-// Sums over the pieces, in their order: the first `count` to out, the next ones to
-// `second`.
-__global__ __launch_bounds__(256) void
-join_sum_kernel(const float *part, int pieces, int64_t stride, int64_t count,
-                int dtype, void *out, void *second) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= stride)
+// Rows of dq (SECOND: of dk, then of dv) as sums over the pieces, in their order: 32
+// lanes a row.
+template <bool SECOND>
+__global__ __launch_bounds__(256) void join_sum_kernel(AttentionCall c,
+                                                       int dtype) {
+  const int keys = c.nk * c.hk;
+  const int rows = SECOND ? 2 * keys : c.nq * c.hq;
+  const int row = blockIdx.x * 8 + threadIdx.x / 32;
+  const int e0 = (threadIdx.x & 31) * 4;
+  if (row >= rows || e0 >= c.d)
     return;
-  float v = 0.f;
+  const int at = SECOND && row >= keys ? row - keys : row;
+  int pieces;
+  if (SECOND) {
+    const int key = at / c.hk, tiles = (c.nk + c.rows - 1) / c.rows;
+    pieces = c.pieces[(at - key * c.hk) * tiles + key / c.rows];
+  } else {
+    pieces = pieces_of(c, at);
+  }
+  if (pieces <= 1)
+    return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < pieces; ++s)
-    v += part[s * stride + i];
-  if (i < count)
-    put_as(dtype, out, i, v);
-  else
-    put_as(dtype, second, i - count, v);
+  for (int s = 0; s < pieces; ++s) {
+    const float *from = c.part + ((int64_t)s * rows + row) * c.d + e0;
+    if (c.d % 4 == 0) {
+      float x[4];
+      __builtin_memcpy(x, __builtin_assume_aligned(from, 16), 16);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] += x[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        v[e] += e0 + e < c.d ? from[e] : 0.f;
+    }
+  }
+  void *out = !SECOND ? c.dq : row < keys ? c.dk : c.dv;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (e0 + e < c.d)
+      put_as(dtype, out, (int64_t)at * c.d + e0 + e, v[e]);
 }
 
 AttentionLauncher launcher(int dtype, int d) {
@@ -225,106 +261,128 @@ AttentionLauncher launcher(int dtype, int d) {
 #undef PCA_BY_WIDTH
 }
 
-hipError_t join_sum(const AttentionCall &c, int64_t stride, int64_t count,
-                    int dtype, void *out, void *second, hipStream_t stream) {
-  const int64_t blocks = (stride + 255) / 256;
-  if (blocks > INT32_MAX)
-    return hipErrorInvalidValue;
-  join_sum_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
-      c.part, c.splits, stride, count, dtype, out, second);
-  return hipGetLastError();
+unsigned join_blocks(int64_t rows, int per) {
+  return (unsigned)((rows + per - 1) / per);
 }
+
+int element_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
 } // namespace
 
 AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
-                             int d) {
+                             int size, int d) {
   const int64_t rows_q = nq * (hq / hk);
   const int64_t owned = pass == 2 ? nk : rows_q;
   const int64_t looped = pass == 2 ? rows_q : nk;
   auto groups = [&](int rows) { return (owned + rows - 1) / rows * hk; };
   AttentionPlan p;
-  p.rows = most_rows(pass, d);
-  if (d <= 32 || (d <= 64 && pass != 2) || groups(p.rows) < 512)
+  p.rows = most_rows(pass, size, d);
+  if (d <= 32 || (d <= 64 && pass != 2 && size == 2) || groups(p.rows) < 512)
     p.rows = 64;
   if (owned <= 256)
     p.rows = kFewRows;
   const int64_t n = std::max<int64_t>(1, groups(p.rows));
-  const int64_t want = p.rows == kFewRows ? 512 : n < 800 ? 2048 : 0;
-  p.splits = (int)std::clamp<int64_t>(
-      (want + n / 2) / n, 1, std::clamp<int64_t>(looped / 128, 1, 64));
+  const int64_t want = p.rows == kFewRows                  ? 512
+                       : n < (p.rows == 128 ? 512 : 800) ? 2048
+                                                           : 0;
+  const int64_t most = looped / least_rows(size, p.rows == kFewRows ? 4 : 1);
+  p.splits = (int)std::clamp<int64_t>((want + n / 2) / n, 1,
+                                      std::clamp<int64_t>(most, 1, 64));
   return p;
 }
 
-static size_t part_bytes(int pass, int64_t nq, int64_t nk, int hq, int hk,
-                         int d) {
-  const int splits = attention_plan(pass, nq, nk, hq, hk, d).splits;
-  if (splits <= 1)
+// Where the pieces' results lie behind `base` (pass as in the plan); returns the bytes.
+static size_t lay_out(AttentionCall &c, int pass, const AttentionPlan &p,
+                      char *base) {
+  c.rows = p.rows;
+  c.splits = p.splits;
+  if (p.splits <= 1)
     return 0;
-  const int64_t one = pass == 2 ? 2 * nk * hk * d : nq * hq * d;
-  size_t bytes = attn_align(sizeof(float) * (size_t)(splits * one));
+  const int64_t owned = pass == 2 ? c.nk : (int64_t)c.nq * (c.hq / c.hk);
+  const int64_t tiles = (owned + p.rows - 1) / p.rows;
+  const int64_t rows =
+      pass == 2 ? 2 * (int64_t)c.nk * c.hk : (int64_t)c.nq * c.hq;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    char *q = base + at;
+    at += attn_align(bytes);
+    return q;
+  };
+  c.part = reinterpret_cast<float *>(
+      take(sizeof(float) * (size_t)(p.splits * rows * c.d)));
+  c.pieces = reinterpret_cast<int *>(take(sizeof(int) * (size_t)(tiles * c.hk)));
   if (pass == 0)
-    bytes += attn_align(sizeof(float) * 2 * (size_t)(splits * nq * hq));
-  return bytes;
+    c.part_ml =
+        reinterpret_cast<float *>(take(sizeof(float) * 2 * p.splits * rows));
+  return at;
 }
 
-size_t attention_workspace_bytes(int pass, int64_t nq, int64_t nk, int hq,
+size_t attention_workspace_bytes(int backward, int64_t nq, int64_t nk, int hq,
                                  int hk, int d) {
-  if (pass == 0)
-    return 256 + part_bytes(0, nq, nk, hq, hk, d);
-  return 2 * attn_align(sizeof(float) * (size_t)(nq * hq)) +
-         attn_align(sizeof(float) * (size_t)hq) + 256 +
-         std::max(part_bytes(1, nq, nk, hq, hk, d),
-                  part_bytes(2, nq, nk, hq, hk, d));
+  AttentionCall c;
+  c.nq = (int)nq;
+  c.nk = (int)nk;
+  c.hq = hq;
+  c.hk = hk;
+  c.d = d;
+  size_t most = 0;
+  for (int pass = backward ? 1 : 0; pass <= (backward ? 2 : 0); ++pass)
+    for (int size : {2, 4}) // (the same for all element types)
+      most = std::max(
+          most, lay_out(c, pass, attention_plan(pass, nq, nk, hq, hk, size, d),
+                        nullptr));
+  if (backward)
+    most += 2 * attn_align(sizeof(float) * (size_t)(nq * hq)) +
+            attn_align(sizeof(float) * (size_t)hq);
+  return most + 256;
 }
 
 hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
                              hipStream_t stream) {
-  const AttentionPlan p = attention_plan(0, c.nq, c.nk, c.hq, c.hk, c.d);
-  c.splits = p.splits;
-  c.part = static_cast<float *>(workspace);
-  c.part_ml = c.part + attn_align(sizeof(float) * (size_t)p.splits * c.nq *
-                                  c.hq * c.d) /
-                           sizeof(float);
-  hipError_t e = launcher(dtype, c.d)(c, 0, p.rows, stream);
+  const AttentionPlan p = attention_plan(0, c.nq, c.nk, c.hq, c.hk,
+                                         element_size(dtype), c.d);
+  lay_out(c, 0, p, static_cast<char *>(workspace));
+  const hipError_t e = launcher(dtype, c.d)(c, 0, p.rows, stream);
   if (e != hipSuccess || p.splits == 1 || c.nq == 0)
     return e;
   // (rows alone fill the chip: a group a row)
-  const int shares = (int64_t)c.nq * c.hq >= 8192 ? 1
-                     : p.splits >= 32             ? 8
-                     : p.splits >= 4              ? 4
-                                                  : 1;
-  const int64_t blocks =
-      ((int64_t)c.nq * c.hq + 8 / shares - 1) / (8 / shares);
-  join_forward_kernel<<<dim3((unsigned)blocks), dim3(256), 0, stream>>>(
-      c, dtype, shares);
+  const int64_t rows = (int64_t)c.nq * c.hq;
+  const int shares = rows >= 8192       ? 1
+                     : p.splits >= 32   ? 8
+                     : p.splits >= 4    ? 4
+                                        : 1;
+  join_forward_kernel<<<dim3(join_blocks(rows, 8 / shares)), dim3(256), 0,
+                        stream>>>(c, dtype, shares);
   return hipGetLastError();
 }
 
 hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
                               hipStream_t stream) {
-  const size_t one =
-      attn_align(sizeof(float) * (size_t)c.nq * c.hq) / sizeof(float);
-  c.minus_delta = static_cast<float *>(workspace);
-  c.base = c.minus_delta + one;
-  c.minus_slope = c.base + one;
-  c.part =
-      c.minus_slope + attn_align(sizeof(float) * (size_t)c.hq) / sizeof(float);
-  const AttentionPlan pq = attention_plan(1, c.nq, c.nk, c.hq, c.hk, c.d);
-  c.splits = pq.splits;
+  const size_t one = attn_align(sizeof(float) * (size_t)c.nq * c.hq);
+  char *base = static_cast<char *>(workspace);
+  c.minus_delta = reinterpret_cast<float *>(base);
+  c.base = reinterpret_cast<float *>(base + one);
+  c.minus_slope = reinterpret_cast<float *>(base + 2 * one);
+  base += 2 * one + attn_align(sizeof(float) * (size_t)c.hq);
+  const int size = element_size(dtype);
+  const AttentionPlan pq = attention_plan(1, c.nq, c.nk, c.hq, c.hk, size, c.d);
+  lay_out(c, 1, pq, base);
   hipError_t e = launcher(dtype, c.d)(c, 1, pq.rows, stream);
-  if (e == hipSuccess && c.splits > 1 && c.nq > 0) {
-    const int64_t count = (int64_t)c.nq * c.hq * c.d;
-    e = join_sum(c, count, count, dtype, c.dq, nullptr, stream);
+  if (e == hipSuccess && pq.splits > 1 && c.nq > 0) {
+    join_sum_kernel<false>
+        <<<dim3(join_blocks((int64_t)c.nq * c.hq, 8)), dim3(256), 0, stream>>>(
+            c, dtype);
+    e = hipGetLastError();
   }
   if (e != hipSuccess)
     return e;
-  const AttentionPlan pk = attention_plan(2, c.nq, c.nk, c.hq, c.hk, c.d);
-  c.splits = pk.splits;
+  const AttentionPlan pk = attention_plan(2, c.nq, c.nk, c.hq, c.hk, size, c.d);
+  lay_out(c, 2, pk, base);
   e = launcher(dtype, c.d)(c, 2, pk.rows, stream);
-  if (e == hipSuccess && c.splits > 1 && c.nk > 0) {
-    const int64_t count = (int64_t)c.nk * c.hk * c.d;
-    e = join_sum(c, 2 * count, count, dtype, c.dk, c.dv, stream);
+  if (e == hipSuccess && pk.splits > 1 && c.nk > 0) {
+    join_sum_kernel<true><<<dim3(join_blocks(2 * (int64_t)c.nk * c.hk, 8)),
+                            dim3(256), 0, stream>>>(c, dtype);
+    e = hipGetLastError();
   }
   return e;
 }

@@ -40,8 +40,11 @@ struct AttentionCall {
   // relative to ([hq, nq]), -slope log2 e ([hq])
   float *minus_delta = nullptr, *base = nullptr, *minus_slope = nullptr;
 
-  // the looped side cut into pieces that meet in a kernel of their own
+  // the looped side cut into up to `splits` pieces that meet in a kernel of their own
   int splits = 1;
+  int rows = 0;             // owned rows of a workgroup
+  int *pieces = nullptr;    // [hk, tiles of owned rows]: in use; 1: the result is
+                            // written already
   float *part = nullptr;    // forward, dq: [splits, nq, hq, d]; dk, dv:
                             // [splits, 2, nk, hk, d]
   float *part_ml = nullptr; // forward: [splits, nq, hq, 2]
@@ -78,13 +81,18 @@ PCA_ATTENTION_DECLARE(bf16);
 // many.  Two blocks of 16 columns per wave share every left operand; where the sums of
 // both do not fit the registers of two waves per SIMD it is one.
 constexpr int kFewRows = 16;
-constexpr int most_rows(int pass, int width) {
-  return width > 64 && pass > 0 ? 64 : 128;
+constexpr int most_rows(int pass, int size, int width) {
+  return width > 64 && (pass > 0 || size == 4) ? 64 : 128;
+}
+
+// Looped rows of a piece, at least (waves: that share the owned rows).
+constexpr int least_rows(int size, int waves) {
+  return size == 4 ? 128 : 512;
 }
 
 AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
-                             int d);
-size_t attention_workspace_bytes(int pass, int64_t nq, int64_t nk, int hq,
+                             int size, int d);
+size_t attention_workspace_bytes(int backward, int64_t nq, int64_t nk, int hq,
                                  int hk, int d);
 // workspace: of attention_workspace_bytes(0, ...) / (1, ...)
 hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,

@@ -450,7 +450,7 @@ template <int ROWS> struct Walk {
   int left, round, count, span, first, begin, end, tile;
   __device__ __forceinline__ Walk(const Spans<ROWS> &spans, int rounds,
                                   int piece, int pieces, int tile_rows)
-      : s(spans), round(0), span(0), first(0), begin(0), end(0),
+      : s(spans), left(0), round(0), span(0), first(0), begin(0), end(0),
         tile(tile_rows) {
     count = __builtin_amdgcn_readfirstlane(s.count);
     const int once =
@@ -494,8 +494,9 @@ template <int ROWS> struct Walk {
 // of the looped rows.  Workgroups of an XCD (every eighth) take neighbouring tiles of
 // the same key head: they read the same rows, through one L2.
 struct Place {
-  int tile, head, piece;
-  __device__ __forceinline__ Place(int tiles, int heads, int pieces) {
+  int tile, head, piece, tiles;
+  __device__ __forceinline__ Place(int number, int heads, int pieces)
+      : tiles(number) {
     // (blocks of an XCD: a grid that is no multiple of 8 leaves the first ones one
     // more)
     const int grid = tiles * heads * pieces, x = blockIdx.x & 7;
@@ -517,6 +518,27 @@ template <typename T, int WK> struct Looped {
                                       : (sizeof(T) == 2 ? 32 : 16);
   static constexpr int tile = wave * WK;
 };
+
+// Pieces that the looped rows of a tile of owned rows [first, last] are cut into, up to
+// c.splits: as many as leave each some tiles (least_rows), so that short examples stay
+// whole and long ones are shared, whatever is next to them.  Known from two spans; the
+// workgroups of the others end at once.
+template <typename T, int WK>
+__device__ __forceinline__ int
+pieces_in_use(const AttentionCall &c, const int2 *spans, int first, int last,
+              int all, int rounds, const Place &place) {
+  if (c.splits == 1)
+    return 1;
+  int rows = all;
+  if (spans)
+    rows = __builtin_amdgcn_readfirstlane(spans[last].y - spans[first].x);
+  const int n = min(
+      max((int)((int64_t)rows * rounds / least_rows(sizeof(T), WK)), 1),
+      c.splits);
+  if (place.piece == 0 && threadIdx.x == 0)
+    c.pieces[place.head * place.tiles + place.tile] = n;
+  return n;
+}
 
 // A lane's owned column.
 struct Column {
@@ -743,6 +765,11 @@ attention_forward_kernel(AttentionCall c) {
   const int wq = wave / WK;
   const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS;
+  const int pieces =
+      pieces_in_use<T, WK>(c, c.spans_q, row0 / group,
+                           (min(row0 + ROWS, rows) - 1) / group, c.nk, 1, place);
+  if (place.piece >= pieces)
+    return; // (the whole workgroup)
 
   Column col[RB];
   u32x4 q[RB][S::KS];
@@ -784,7 +811,7 @@ attention_forward_kernel(AttentionCall c) {
   if (c.d < S::LDS)
     clear_lds<4 * TILE>(lds_tiles);
 
-  Walk<ROWS> walk(spans, 1, place.piece, c.splits, KT);
+  Walk<ROWS> walk(spans, 1, place.piece, pieces, KT);
   int buffer = 0;
   Members<RB> members;
   if (walk.there())
@@ -967,7 +994,7 @@ attention_forward_kernel(AttentionCall c) {
     const int64_t at = (int64_t)col[rb].row * c.hq + col[rb].head;
     const bool vec = c.d % 4 == 0;
     const bool first = g == 0 && (WK == 1 || wave == 0);
-    if (c.splits > 1) {
+    if (pieces > 1) {
       const int64_t o = (int64_t)place.piece * c.nq * c.hq + at;
 #pragma unroll
       for (int db = 0; db < S::DB; ++db) {
@@ -1101,6 +1128,11 @@ __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void att
   const int wq = wave / WK;
   const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS;
+  const int pieces =
+      pieces_in_use<T, WK>(c, c.spans_q, row0 / group,
+                           (min(row0 + ROWS, rows) - 1) / group, c.nk, 1, place);
+  if (place.piece >= pieces)
+    return; // (the whole workgroup)
 
   Column col[RB];
   u32x4 q[RB][S::KS], dout[RB][S::KS];
@@ -1180,7 +1212,7 @@ __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void att
   if (c.d < S::LDS)
     clear_lds<4 * TILE>(lds_tiles);
 
-  Walk<ROWS> walk(spans, 1, place.piece, c.splits, KT);
+  Walk<ROWS> walk(spans, 1, place.piece, pieces, KT);
   int buffer = 0;
   Members<RB> members;
   if (walk.there())
@@ -1318,7 +1350,7 @@ __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void att
     if (col[rb].valid) {
       const int64_t at = (int64_t)col[rb].row * c.hq + col[rb].head;
       float *piece =
-          c.splits > 1
+          pieces > 1
               ? c.part + (int64_t)place.piece * c.nq * c.hq * c.d
               : nullptr;
       store_columns<T, DP, RB, WK>(acc, rb, c.dq, piece, at, c.d,
@@ -1348,6 +1380,11 @@ attention_dkv_kernel(AttentionCall c) {
   const int wq = wave / WK;
   const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS, head0 = place.head * group;
+  const int pieces =
+      pieces_in_use<T, WK>(c, c.spans_k, row0, min(row0 + ROWS, c.nk) - 1, c.nq,
+                           group, place);
+  if (place.piece >= pieces)
+    return; // (the whole workgroup)
 
   Column col[RB];
   u32x4 k[RB][S::KS], v[RB][S::KS];
@@ -1398,7 +1435,7 @@ attention_dkv_kernel(AttentionCall c) {
   if (c.d < S::LDS)
     clear_lds<4 * TILE>(lds_tiles);
 
-  Walk<ROWS> walk(spans, group, place.piece, c.splits, KT);
+  Walk<ROWS> walk(spans, group, place.piece, pieces, KT);
   int buffer = 0;
   Members<RB> members;
   if (walk.there())
@@ -1578,7 +1615,7 @@ attention_dkv_kernel(AttentionCall c) {
     if (col[rb].valid) {
       const int64_t at = (int64_t)col[rb].row * c.hk + place.head;
       const int64_t one = (int64_t)c.nk * c.hk * c.d;
-      float *piece = c.splits > 1 ? c.part + place.piece * 2 * one : nullptr;
+      float *piece = pieces > 1 ? c.part + place.piece * 2 * one : nullptr;
       store_columns<T, DP, RB, WK>(acc_k, rb, c.dk, piece, at, c.d,
                                    c.cap > 0.f ? c.scale * kFlatUp<T> : c.scale);
       store_columns<T, DP, RB, WK>(acc_v, rb, c.dv, piece ? piece + one : nullptr,
@@ -1607,11 +1644,11 @@ hipError_t launch(const AttentionCall &c, int pass, int rows,
   else                                                                         \
     kernel<T, DP, most / 64, 1><<<g, b, 0, stream>>>(c)
   if (pass == 0) {
-    PCA_LAUNCH(attention_forward_kernel, most_rows(0, DP));
+    PCA_LAUNCH(attention_forward_kernel, most_rows(0, sizeof(T), DP));
   } else if (pass == 1) {
-    PCA_LAUNCH(attention_dq_kernel, most_rows(1, DP));
+    PCA_LAUNCH(attention_dq_kernel, most_rows(1, sizeof(T), DP));
   } else {
-    PCA_LAUNCH(attention_dkv_kernel, most_rows(2, DP));
+    PCA_LAUNCH(attention_dkv_kernel, most_rows(2, sizeof(T), DP));
   }
 #undef PCA_LAUNCH
   return hipGetLastError();
