@@ -31,7 +31,7 @@ extern "C" {
 /*
  * spans[2 i], spans[2 i + 1] = first row of b whose example id is that of row
  * i of a, first row behind them (ids sorted; equal if b has none): which rows
- * of b belong to row i.  spans: [2 na] int32.
+ * of b belong to row i.  spans: [2 na] int32, on 8 bytes.
  */
 int pca_spans(const int64_t *ids_a, int64_t na, const int64_t *ids_b,
               int64_t nb, int32_t *spans, void *stream);

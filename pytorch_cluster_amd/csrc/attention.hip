@@ -285,7 +285,7 @@ AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
   const int64_t want = p.rows == kFewRows                  ? 512
                        : n < (p.rows == 128 ? 512 : 800) ? 2048
                                                            : 0;
-  const int64_t most = looped / least_rows(size, p.rows == kFewRows ? 4 : 1);
+  const int64_t most = looped / least_rows(size);
   p.splits = (int)std::clamp<int64_t>((want + n / 2) / n, 1,
                                       std::clamp<int64_t>(most, 1, 64));
   return p;

@@ -523,7 +523,7 @@ template <typename T, int WK> struct Looped {
 // c.splits: as many as leave each some tiles (least_rows), so that short examples stay
 // whole and long ones are shared, whatever is next to them.  Known from two spans; the
 // workgroups of the others end at once.
-template <typename T, int WK>
+template <typename T>
 __device__ __forceinline__ int
 pieces_in_use(const AttentionCall &c, const int2 *spans, int first, int last,
               int all, int rounds, const Place &place) {
@@ -533,7 +533,7 @@ pieces_in_use(const AttentionCall &c, const int2 *spans, int first, int last,
   if (spans)
     rows = __builtin_amdgcn_readfirstlane(spans[last].y - spans[first].x);
   const int n = min(
-      max((int)((int64_t)rows * rounds / least_rows(sizeof(T), WK)), 1),
+      max((int)((int64_t)rows * rounds / least_rows(sizeof(T))), 1),
       c.splits);
   if (place.piece == 0 && threadIdx.x == 0)
     c.pieces[place.head * place.tiles + place.tile] = n;
@@ -766,7 +766,7 @@ attention_forward_kernel(AttentionCall c) {
   const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS;
   const int pieces =
-      pieces_in_use<T, WK>(c, c.spans_q, row0 / group,
+      pieces_in_use<T>(c, c.spans_q, row0 / group,
                            (min(row0 + ROWS, rows) - 1) / group, c.nk, 1, place);
   if (place.piece >= pieces)
     return; // (the whole workgroup)
@@ -938,12 +938,11 @@ attention_forward_kernel(AttentionCall c) {
   }
 
 #pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
-    if (!seen[rb])
-      m[rb] = -__builtin_inff(); // nothing to be put together with others
-#pragma unroll
-  for (int rb = 0; rb < RB; ++rb)
+  for (int rb = 0; rb < RB; ++rb) {
     l[rb] = across_groups_sum(l[rb]);
+    if (!seen[rb] && l[rb] == 0.f) // (not: scores that were all NaN)
+      m[rb] = -__builtin_inff();   // nothing to be put together with others
+  }
 
   if constexpr (WK > 1) {
     // the waves' shares of the same 16 columns: one maximum, then sums in the order
@@ -1129,7 +1128,7 @@ __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void att
   const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS;
   const int pieces =
-      pieces_in_use<T, WK>(c, c.spans_q, row0 / group,
+      pieces_in_use<T>(c, c.spans_q, row0 / group,
                            (min(row0 + ROWS, rows) - 1) / group, c.nk, 1, place);
   if (place.piece >= pieces)
     return; // (the whole workgroup)
@@ -1381,7 +1380,7 @@ attention_dkv_kernel(AttentionCall c) {
   const int part = __builtin_amdgcn_readfirstlane(wave % WK * KW);
   const int row0 = place.tile * ROWS, head0 = place.head * group;
   const int pieces =
-      pieces_in_use<T, WK>(c, c.spans_k, row0, min(row0 + ROWS, c.nk) - 1, c.nq,
+      pieces_in_use<T>(c, c.spans_k, row0, min(row0 + ROWS, c.nk) - 1, c.nq,
                            group, place);
   if (place.piece >= pieces)
     return; // (the whole workgroup)
@@ -1633,7 +1632,7 @@ hipError_t launch(const AttentionCall &c, int pass, int rows,
   const int64_t grid = (owned + rows - 1) / rows * c.hk * c.splits;
   if (grid <= 0)
     return hipSuccess;
-  if (grid > INT32_MAX)
+  if (grid * kThreads > UINT32_MAX) // (what a launch can number)
     return hipErrorInvalidValue;
   const dim3 g((unsigned)grid), b(kThreads);
 #define PCA_LAUNCH(kernel, most)                                               \

@@ -86,6 +86,11 @@ int attention_call(const pca_attention_args *a, pca::AttentionCall &c) {
        (a->nk > 0 && a->pos_k == nullptr)))
     return pca::fail(PCA_ERR_INVALID_ARGUMENT,
                      "attention: a slope needs positions of 1 to 3 axes");
+  if (((reinterpret_cast<uintptr_t>(a->spans_q) |
+        reinterpret_cast<uintptr_t>(a->spans_k)) &
+       7) != 0)
+    return pca::fail(PCA_ERR_INVALID_ARGUMENT,
+                     "attention: spans have to start on 8 bytes");
   if (!std::isfinite(a->scale) || !std::isfinite(a->cap) || a->cap < 0.f)
     return pca::fail(PCA_ERR_INVALID_ARGUMENT,
                      "attention: scale and cap have to be finite, cap not "

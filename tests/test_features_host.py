@@ -144,6 +144,7 @@ def test_c_abi_checks_before_any_launch():
     assert forward(cap=-1.0) == -1
     assert forward(scale=float("nan")) == -1
     assert forward(out=at + 8) == -1
+    assert forward(spans_q=at + 4) == -1
     assert forward(size=16) == -3
     assert forward(ws=at + 8) == -3
     assert forward(ws=None) == -3

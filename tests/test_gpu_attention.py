@@ -206,6 +206,18 @@ def test_scores_that_overflow():
     assert torch.isfinite(out[keep]).all()
 
 
+@pytest.mark.parametrize("nq, nk", [(1, 70), (3, 9000), (80, 50), (300, 9000)])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_scores_that_are_not_numbers(dtype, nq, nk):
+    # all scores of a row, in every piece that its keys are cut into
+    x = inputs(5, nq, nk, 1, 1, 32, TYPES[dtype], dout=False)
+    x["q"][nq // 2, 0, 3] = float("nan")
+    out = call(x)["out"]
+    assert torch.isnan(out[nq // 2]).all()
+    keep = torch.arange(nq, device=DEV) != nq // 2
+    assert torch.isfinite(out[keep]).all()
+
+
 def test_all_scores_minus_infinity():
     x = inputs(4, 20, 50, 1, 1, 16, torch.float32, axes=1, dout=False)
     x["pos_q"][3] = float("inf")
