@@ -61,7 +61,8 @@ __device__ __forceinline__ int wave_bound_of(const int64_t *ids, int n,
 // spans[i] = [first row of b with row i's id, first one with a larger id).  The waves
 // of a workgroup find where its first and its last id lie, three dependent reads for
 // 200,000 rows; only workgroups with rows of several examples search further, between
-// the two.
+// the two.  Latency alone: 2.4 us for one example of 1,024 rows, 5.4 us for a thousand
+// examples in 35,000 rows, 7.5 us for 32 queries among 143,000 rows.
 __global__ __launch_bounds__(256) void spans_kernel(const int64_t *ids_a, int na,
                                                     const int64_t *ids_b,
                                                     int nb, int2 *spans) {
@@ -120,9 +121,14 @@ __device__ __forceinline__ int pieces_of(const AttentionCall &c, int row) {
   return c.pieces[kv * tiles + (query * group + head - kv * group) / c.rows];
 }
 
-// Output rows from the pieces' sums, maxima and sums of weights: 32 lanes take four
-// elements each; where there are many pieces, `shares` groups of lanes divide them and
-// meet in LDS, in their order.
+// Output rows from the pieces' sums, maxima and sums of weights,
+//
+//   o = sum_s 2^(m_s - m) acc_s / sum_s 2^(m_s - m) l_s,   m = max_s m_s:
+//
+// 32 lanes take four elements each; where there are many pieces, `shares` groups of lanes
+// divide them and meet in LDS, in their order.  Four ragged
+// scans, up to 1,024 queries each of 8 heads of 64, up to 8 pieces: 13 us; 256 rows of 128
+// in up to 64 pieces: 7 us, latency.
 __global__ __launch_bounds__(256) void
 join_forward_kernel(AttentionCall c, int dtype, int shares) {
   __shared__ float lds_acc[8][128], lds_ml[8][2];
@@ -269,6 +275,22 @@ int element_size(int dtype) { return dtype == 0 ? 4 : 2; }
 
 } // namespace
 
+// Rows of a workgroup (both sides measured, us; bf16 where nothing else is said).  128 or
+// 64 rows: heads of 64 with a bias, forward, 16 x 1,024 rows of 8 heads 118 / 106, 4 x 4,096
+// rows 365 / 317 (four waves per SIMD cover the distances), forward and backward with
+// dk / dv at 128 and 64 rows 235 / 260, fp32 306 / 337; heads of 32, a thousand graphs of 35
+// rows on average, all three kernels 183 / 120.  64 rows as well if 128 leave a CU less
+// than two workgroups.  16 rows, whose waves divide the keys, or 64, with their joins: 32
+// single queries 43 / 54, one cloud of 1,024 rows 24 / 25, four ragged scans with 1,024
+// queries each at most 131 / 85.
+//
+// Pieces of the looped side where workgroups are few (about three to a CU; those of 128
+// rows never are): 2,048 workgroups' worth.  12 ragged examples in fp32, one to eight
+// pieces: 756, 640, 589, 623; four ragged scans, one, four, eight: 269, 100, 92; from
+// 1,024 workgroups on pieces lose (clouds, one and two: 384, 497).  With 16 rows a
+// workgroup 512 workgroups' worth (32 queries, 16 to 128 pieces: 58, 60, 71, 97).  How many
+// of the pieces a tile of rows uses goes by the length of its own examples
+// (pieces_in_use).
 AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
                              int size, int d) {
   const int64_t rows_q = nq * (hq / hk);
@@ -282,9 +304,9 @@ AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
   if (owned <= 256)
     p.rows = kFewRows;
   const int64_t n = std::max<int64_t>(1, groups(p.rows));
-  const int64_t want = p.rows == kFewRows                  ? 512
-                       : n < (p.rows == 128 ? 512 : 800) ? 2048
-                                                           : 0;
+  const int64_t want = p.rows == kFewRows             ? 512
+                       : p.rows == 64 && n < 800 ? 2048
+                                                      : 0;
   const int64_t most = looped / least_rows(size);
   p.splits = (int)std::clamp<int64_t>((want + n / 2) / n, 1,
                                       std::clamp<int64_t>(most, 1, 64));

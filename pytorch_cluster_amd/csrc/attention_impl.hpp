@@ -35,7 +35,24 @@
 // that hold nothing of another example (rows beyond it are zeros), and where a wave's
 // columns belong to several examples the products are kept only in the columns that
 // the span belongs to: values of other examples, infinities and NaN among them, reach
-// nothing.
+// nothing.  A tile costs 2.0 - 2.5 us of latency in a workgroup however few rows of it
+// a span fills, so examples of a few rows pay for tiles of 64: 303 graphs of 6 rows take
+// 91 us.  Neighbouring short spans in one tile, masked lane by lane, took 31 us there,
+// but the masks' registers cost the long examples 10 - 24 % and were taken back.
+//
+// What bounds them (one MI355X; 16 clouds of 1,024 rows, 8 heads of 64, bf16, positions
+// on three axes): the vector unit.  64 pairs of rows cost 17 - 19 vector instructions
+// (distance 7; exponential and square root at a quarter of the rate).  Forward 104 us, the
+// vector unit busy for 81 % of the cycles and the matrix cores for 17; dq 120 us, 67 and
+// 21 %; dk and dv 151 us, 54 and 21 %, with two waves per SIMD, which no longer cover
+// each other's products, exchanges and barriers.  Without bias and cap the forward
+// reaches 938 TFLOP/s with heads of 128 (4 examples of 4,096 rows, 8 heads, bf16: 293
+// us) and 681 with heads of 64, forward and backward 668 and 631 (a product of 8,192^3:
+// 1,261); fp32, where the matrix cores are busy for half of the cycles, 112 - 116 of 153.
+//
+// Tiles come by loads that bypass the registers (request16), one tile ahead: with loads
+// into registers and stores to LDS 4 examples of 4,096 rows with everything on took 1,312
+// / 1,375 / 1,833 us instead of 576 / 680 / 964 (now 485 / 654 / 855).
 #pragma once
 
 #include "attention.hpp"
@@ -93,14 +110,17 @@ template <typename T, int DP> struct Shape {
   static constexpr int KF = SZ == 2 ? 32 : 16; // rows of a step over rows
   static constexpr int FB = KF / 16;           // ... in blocks
   // A tile's rows lie in LDS one after the other, as the loads that bypass the
-  // registers leave them.  Piece p of row r is kept at place p ^ turn(r): the same
-  // piece of 16 neighbouring rows then lies on 64 different banks, and so do, for
-  // 16-bit elements, pairs of pieces of 8 neighbouring rows (turned_operand).
+  // registers leave them.  Piece p of row r is kept at place p ^ turn(r).  The 16 lanes
+  // that read 16 bytes each at a time are not neighbours: rows 0 - 3 and 12 - 15 of one
+  // piece, 4 - 11 of the next (rows_operand).  With 16-bit elements pairs of pieces of 8
+  // neighbouring rows are read as well (turned_operand).  Both then lie on 64 different
+  // banks; rows r and r + 8 of 16 have to be turned alike for that (told apart they cost
+  // twice the cycles, a third of the LDS's in dq of heads of 128).
   __device__ __forceinline__ static int turn(int row) {
     constexpr int ROWS = CH >= 16 ? 1 : 16 / CH; // that fill the banks
     if (SZ == 4)
       return row / ROWS & (CH >= 16 ? 15 : CH - 1);
-    return (row / ROWS & (CH >= 16 ? 7 : CH / 2 - 1)) << 1 | (row >> 3 & 1);
+    return (row / ROWS & (CH >= 16 ? 7 : CH / 2 - 1)) << 1;
   }
 };
 
@@ -492,7 +512,9 @@ template <int ROWS> struct Walk {
 
 // The work of workgroup `block`: which tile of owned rows, which key head, which piece
 // of the looped rows.  Workgroups of an XCD (every eighth) take neighbouring tiles of
-// the same key head: they read the same rows, through one L2.
+// the same key head: they read the same rows, through one L2.  (Runs of 8 to 32
+// workgroups dealt to the XCDs by turns: 79 us instead of 71 where long and short
+// examples follow each other.)
 struct Place {
   int tile, head, piece, tiles;
   __device__ __forceinline__ Place(int number, int heads, int pieces)
@@ -507,12 +529,19 @@ struct Place {
   }
 };
 
-// Waves per SIMD that the registers are cut to.
+// Waves per SIMD that the registers are cut to: four where the sums of one block of
+// columns leave room for them (five or six for heads of 32 were no faster), else two; the
+// waves that divide tiles of wide heads among them come one to a SIMD, and LDS holds no
+// more of them anyway.
 template <typename T, int DP, int RB, int WK> constexpr int waves_wanted() {
-  return WK > 1 && DP > 64 ? 1 : sizeof(T) == 2 && DP <= 64 && RB == 1 && WK == 1 ? 4 : 2;
+  if (WK > 1)
+    return DP > 64 ? 1 : 2;
+  return sizeof(T) == 2 && DP <= 64 && RB == 1 ? 4 : 2;
 }
 
 // Rows of looped tiles per wave and step: the tile's 16-byte pieces fill the threads.
+// (Tiles of 32 rows for 16-bit heads of 128, so that two workgroups share a CU's LDS, were
+// slower: forward 609 us against 575, dk and dv 1,110 against 908.)
 template <typename T, int WK> struct Looped {
   static constexpr int wave = WK == 1 ? (sizeof(T) == 2 ? 64 : 32)
                                       : (sizeof(T) == 2 ? 32 : 16);
@@ -745,6 +774,17 @@ __device__ __forceinline__ void take_distance(f32x4 (&s)[RB][NB],
 
 // Rows of a wave's columns: RB blocks of 16.  WK waves share the same columns and
 // divide every tile among them (few rows); the others own columns of their own.
+//
+// One pass over the keys: with m what is subtracted so far, l the weights' sum,
+//
+//   l' = l 2^(m - m') + sum_j 2^(s_j - m')     o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j
+//
+// where m' differs from m only if a score is above m by more than 8: weights are then at
+// most 256, in 32-bit sums, and nearly all tiles skip the scaling.
+//
+// Bound by the vector unit (see above) where rows are many; by latency where they are
+// few: one cloud of 1,024 rows, 4 heads of 32, fp32, in pieces, 17 us; 32 single queries
+// over 8,192 rows at most, 2 key heads of 128, bf16, 35 us = 4.2 TB/s of keys and values.
 template <typename T, int DP, int RB, int WK>
 __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void
 attention_forward_kernel(AttentionCall c) {
@@ -1109,8 +1149,17 @@ store_columns(const Sums<T, DP, RB> &acc, int rb, void *out, float *part,
 
 // dq of the rows that a workgroup owns, looping over keys; writes what the kernel of dk
 // and dv takes of a row.
+//
+// Scores are formed again (P = 2^(s - lse): no memory for them), three products a pair.
+// -delta is what the product with v starts from.  A step is as many rows as the matrix
+// instruction's contraction, so that scores and dP of a step alone hold registers.  4 x
+// 4,096 rows, 8 heads of 128, bf16, bias and cap: 654 us, 630 TFLOP/s of its three
+// products; vector unit 49 %, matrix cores 28 %, LDS 30 % of the cycles at two waves per
+// SIMD.  One block of columns per wave, since two spill (680 -
+// 1,036 us).
 template <typename T, int DP, int RB, int WK>
-__global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void attention_dq_kernel(AttentionCall c) {
+__global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void
+attention_dq_kernel(AttentionCall c) {
   using S = Shape<T, DP>;
   constexpr int WQ = kWaves / WK, ROWS = RB * 16 * WQ;
   constexpr int KW = Looped<T, WK>::wave, KT = Looped<T, WK>::tile;
@@ -1357,7 +1406,13 @@ __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void att
     }
 }
 
-// dk and dv of the keys that a workgroup owns, looping over (query, head) rows.
+// dk and dv of the keys that a workgroup owns, looping over (query, head) rows, head
+// after head of the group: their gradients add up in the registers, in that order.
+//
+// Four products a pair.  A row's numbers (position, slope, lse, delta) come with its
+// tile.  P goes to dv's product, dT to dk's, both rounded for the matrix cores.  The
+// call above: 855 us, 643 TFLOP/s of its four products; vector unit 43 %, matrix cores
+// 28 %, LDS 35 %.
 template <typename T, int DP, int RB, int WK>
 __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void
 attention_dkv_kernel(AttentionCall c) {
