@@ -19,7 +19,7 @@
 // reads of single rows are what keeps it from the copy's 5.0); gradient: digits 16 + 9
 // + 39 us (count, scan, scatter of two passes), sums 81 us = 4.1 TB/s, joins 9.5 us.
 // 1,048,576 entries of 64 bf16 components, 4,096 rows, a few of which have most entries:
-// forward 23.5 us = 6.0 TB/s (written past the caches), digits 37, sums 38, joins 53 us.
+// forward 23.5 us = 6.0 TB/s (written past the caches), digits 37, sums 38, joins 15 us.
 #include "rows_ops.hpp"
 
 #include "attention_impl.hpp"
@@ -374,19 +374,34 @@ struct Chunks {
 };
 
 // Lanes that take an entry's row, 16 bytes each (wide rows: in columns of LANES pieces,
-// blockIdx.y).  Eight rows are under way per group.
+// blockIdx.y).  Eight rows are under way per group.  A workgroup whose chunks lie inside
+// one run with an entry to spare on both sides leaves one sum for all of them, in the
+// place of its first chunk: a row with 131,000 entries is 4,096 chunks, a megabyte of sums
+// that one workgroup would read for the join (53 us; 15 this way).
 template <typename T, int LANES>
 __global__ __launch_bounds__(256) void
 lookup_sum_kernel(LookupCall c, Sorted s, Chunks k) {
   constexpr int PER = 16 / (int)sizeof(T), GROUPS = 256 / LANES, AHEAD = 8;
-  const int lane = threadIdx.x % LANES;
-  const int64_t chunk = (int64_t)blockIdx.x * GROUPS + threadIdx.x / LANES;
-  const int64_t e0 = ((int64_t)blockIdx.y * LANES + lane) * PER;
-  if (chunk >= k.count || e0 >= c.width)
-    return;
+  __shared__ float part[GROUPS][LANES * PER + 1];
+  const int lane = threadIdx.x % LANES, grp = threadIdx.x / LANES;
+  const int64_t chunk = (int64_t)blockIdx.x * GROUPS + grp;
+  const uint32_t none = (uint32_t)c.table;
+  // (the same in the whole workgroup; sorted keys: all between the two are alike)
+  const int64_t before = (int64_t)blockIdx.x * GROUPS * k.length - 1;
+  const int64_t behind = before + 1 + GROUPS * k.length;
+  const bool inside = before >= 0 && behind < c.entries &&
+                      s.keys[before] == s.keys[behind] &&
+                      s.keys[behind] != none;
+  int64_t e0 = ((int64_t)blockIdx.y * LANES + lane) * PER;
+  if (e0 >= c.width) {
+    if (!inside)
+      return;
+    e0 = 0; // (read, and not written)
+  }
+  if (chunk >= k.count)
+    return; // (not inside)
   const int64_t begin = chunk * k.length;
   const int64_t end = min(begin + k.length, c.entries);
-  const uint32_t none = (uint32_t)c.table;
   const bool vec = c.width % PER == 0;
   uint32_t now = s.keys[begin];
   if (now == none)
@@ -465,11 +480,44 @@ lookup_sum_kernel(LookupCall c, Sorted s, Chunks k) {
       perm[j] = next_perm[j];
     }
   }
-  put(end < c.entries && s.keys[end] == now);
+  if (!inside) {
+    put(end < c.entries && s.keys[end] == now);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i)
+    part[grp][lane * PER + i] = sum[i];
+  __syncthreads();
+  for (int col = threadIdx.x; col < LANES * PER; col += 256) {
+    const int64_t e = (int64_t)blockIdx.y * LANES * PER + col;
+    if (e >= c.width)
+      continue;
+    float all = 0.f;
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j)
+      all += part[j][col];
+    k.ends[(int64_t)blockIdx.x * GROUPS * 2 * c.width + e] = all;
+  }
 }
 
+// The parts of a run that starts in chunk `chunk` and goes on behind it; chunk `stop` is the
+// first that does not begin with its row.  Chunks up to a workgroup's first, workgroups
+// that lie inside the run, chunks behind them.
+template <int GROUPS> struct Parts {
+  int chunk, head, whole, count; // (chunks are far below 2^31)
+  __device__ __forceinline__ Parts(int from, int stop) : chunk(from) {
+    const int next = (int)((unsigned)from / GROUPS + 1) * GROUPS;
+    head = min(next, stop) - from;
+    whole = (int)((unsigned)max(stop - 1 - next, 0) / GROUPS);
+    count = stop - from - whole * (GROUPS - 1);
+  }
+  __device__ __forceinline__ int operator[](int n) const {
+    return chunk + n + (GROUPS - 1) * min(max(n - head, 0), whole);
+  }
+};
+
 // A group of lanes per chunk: where a run starts in it that goes on behind it, the run's
-// parts are added up.  Runs of many chunks (kLong or more) are added up by the whole
+// parts are added up.  Runs of many parts (kLong or more) are added up by the whole
 // workgroup, one after the other: parts dealt to the groups, put together in the order
 // of the groups.
 constexpr int kLong = 16;
@@ -504,7 +552,8 @@ lookup_join_kernel(LookupCall c, Sorted s, Chunks k) {
   {
     const int64_t chunk = (int64_t)blockIdx.x * GROUPS + grp;
     const int64_t begin = chunk * k.length, end = begin + k.length;
-    int64_t stop = 0; // first chunk behind the run; 0: none starts here
+    int64_t stop = 0;
+    bool many = false;
     if (end < c.entries) {
       const uint32_t now = s.keys[end - 1];
       if (now != (uint32_t)c.table && s.keys[end] == now &&
@@ -526,13 +575,20 @@ lookup_join_kernel(LookupCall c, Sorted s, Chunks k) {
             hi = mid;
         }
         stop = hi;
-        if (stop - chunk < kLong && e0 < c.width) {
+        const Parts<GROUPS> parts((int)chunk, (int)stop);
+        many = parts.count >= kLong;
+        if (!many && e0 < c.width) {
           float sum[PER];
 #pragma unroll
           for (int i = 0; i < PER; ++i)
             sum[i] = 0.f;
-          for (int64_t at = chunk; at < stop; ++at)
-            add(sum, chunk, at);
+          if (parts.whole == 0) {
+            for (int64_t at = chunk; at < stop; ++at)
+              add(sum, chunk, at);
+          } else {
+            for (int n = 0; n < parts.count; ++n)
+              add(sum, chunk, parts[n]);
+          }
           T *to = static_cast<T *>(c.out) + (int64_t)now * c.width + e0;
 #pragma unroll
           for (int i = 0; i < PER; ++i)
@@ -542,7 +598,7 @@ lookup_join_kernel(LookupCall c, Sorted s, Chunks k) {
       }
     }
     if (lane == 0)
-      long_stop[grp] = stop - chunk >= kLong ? stop : 0;
+      long_stop[grp] = many ? stop : 0;
   }
   __syncthreads();
   for (int g = 0; g < GROUPS; ++g) {
@@ -554,9 +610,10 @@ lookup_join_kernel(LookupCall c, Sorted s, Chunks k) {
 #pragma unroll
     for (int i = 0; i < PER; ++i)
       sum[i] = 0.f;
+    const Parts<GROUPS> parts((int)chunk, (int)stop);
 #pragma unroll 8
-    for (int64_t at = chunk + grp; at < stop; at += GROUPS)
-      add(sum, chunk, at);
+    for (int n = grp; n < parts.count; n += GROUPS)
+      add(sum, chunk, parts[n]);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < PER; ++i)
