@@ -58,6 +58,13 @@ def test_few_rows_have_most_entries(dtype, skew):
     compare(*inputs(1, 4096, 200000, 24, TYPES[dtype], skew=skew))
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("width", [5, 300, 1000])
+def test_long_runs_of_wide_rows(dtype, width):
+    # workgroups inside one run, in several columns, the last one in part
+    compare(*inputs(8, 40, 30000, width, TYPES[dtype], skew=6.0, none=0.1))
+
+
 def test_all_entries_in_one_row():
     weight, index, dout = inputs(2, 1000, 100000, 32, torch.bfloat16)
     for row in (0, 517, 999):
