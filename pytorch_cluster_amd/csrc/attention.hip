@@ -4,6 +4,7 @@
 #include "attention_impl.hpp"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace pca {
 
@@ -255,6 +256,17 @@ __global__ __launch_bounds__(256) void join_sum_kernel(AttentionCall c,
       put_as(dtype, out, (int64_t)at * c.d + e0 + e, v[e]);
 }
 
+// Numbers that go with the cap, in fp32's range: a cap of 2^127 or more is one of 2^127
+// (cap log2 e is formed, and bends nothing that is not as large), and behind a tiny one
+// products of zero stay zero (and not zero times infinity).
+void set_cap(AttentionCall &c) {
+  if (c.cap <= 0.f)
+    return;
+  c.cap = std::min(c.cap, 0x1p127f);
+  const double in = 2.0 * 1.44269504088896340736 * c.scale / c.cap;
+  c.under_tanh = (float)std::clamp(in, -(double)FLT_MAX, (double)FLT_MAX);
+}
+
 AttentionLauncher launcher(int dtype, int d) {
 #define PCA_BY_WIDTH(type)                                                     \
   (d <= 32   ? attention_##type##_d32                                          \
@@ -361,6 +373,7 @@ size_t attention_workspace_bytes(int backward, int64_t nq, int64_t nk, int hq,
 
 hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
                              hipStream_t stream) {
+  set_cap(c);
   const AttentionPlan p = attention_plan(0, c.nq, c.nk, c.hq, c.hk,
                                          element_size(dtype), c.d);
   lay_out(c, 0, p, static_cast<char *>(workspace));
@@ -380,6 +393,7 @@ hipError_t attention_forward(AttentionCall c, int dtype, void *workspace,
 
 hipError_t attention_backward(AttentionCall c, int dtype, void *workspace,
                               hipStream_t stream) {
+  set_cap(c);
   const size_t one = attn_align(sizeof(float) * (size_t)c.nq * c.hq);
   char *base = static_cast<char *>(workspace);
   c.minus_delta = reinterpret_cast<float *>(base);

@@ -25,6 +25,8 @@ struct AttentionCall {
   int axes = 0;
   int nq = 0, nk = 0, hq = 0, hk = 0, d = 0;
   float scale = 1.f, cap = 0.f;
+  float under_tanh = 0.f; // with a cap: what a product is multiplied by for exp2 in
+                          // tanh, 2 log2 e scale / cap (set_cap)
 
   void *out = nullptr;  // [nq, hq, d], dense
   void *rest = nullptr; // the same: what rounding took off out; or NULL (backward:

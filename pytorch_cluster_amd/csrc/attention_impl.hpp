@@ -379,8 +379,8 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return across_groups(v, [](float a, float b) { return a + b; });
 }
 
-// tanh y for fp32 rows, x = 2 y log2 e: (exp2(x) - 1) / (exp2(x) + 1), and near 0,
-// where that difference would lose digits, the series (error 2e-8 relative below 0.35).
+// tanh y, x = 2 y log2 e: (exp2(x) - 1) / (exp2(x) + 1), and near 0, where that difference
+// would lose digits, the series (error 2e-8 relative below 0.35).
 __device__ __forceinline__ float tanh_of(float x) {
   const float e = __builtin_amdgcn_exp2f(x);
   const float far = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
@@ -664,30 +664,40 @@ __device__ __forceinline__ void add_product(Sums<T, DP, RB> &acc,
 template <typename T>
 constexpr float kFlatUp = std::is_same<T, float>::value ? 1.f : 4.f;
 
+// Up to which cap 16-bit rows take the short form, cap (1 - 2 w) with the cap itself in
+// `base`: an exponential and a reciprocal, but what it rounds is as large as the cap, so
+// a score is off by 1.7e-7 cap: 2e-5 here, a 24th of what rounding a weight to fp16 takes
+// off.  Beyond, and in fp32, a score is as exact as its own size (tanh_of).
+constexpr float kShortCap = 128.f;
+template <typename T>
+__device__ __forceinline__ bool short_cap(const AttentionCall &c) {
+  return !std::is_same<T, float>::value && c.cap <= kShortCap;
+}
+
 // What cap_scores adds to every score: it wants `base` less this.
 template <typename T>
 __device__ __forceinline__ float under_cap(const AttentionCall &c) {
-  return c.cap > 0.f && !std::is_same<T, float>::value ? c.cap * kLog2e : 0.f;
+  return c.cap > 0.f && short_cap<T>(c) ? c.cap * kLog2e : 0.f;
 }
 
-template <typename T, bool FLAT>
+template <typename T, bool SHORT, bool FLAT>
 __device__ __forceinline__ void cap_scores(f32x4 &s, const AttentionCall &c,
                                            f32x4 base, f32x4 *flat) {
-  const float in = c.scale / c.cap * (2.f * kLog2e), out = c.cap * kLog2e;
+  const float in = c.under_tanh, out = c.cap * kLog2e;
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
-    if constexpr (std::is_same<T, float>::value) {
-      const float t = tanh_of(s[r] * in);
-      s[r] = fmaf(t, out, -base[r]);
-      if constexpr (FLAT)
-        (*flat)[r] = fmaf(-t, t, 1.f);
-    } else {
+    if constexpr (SHORT) {
       // tanh = 1 - 2 w (the 1 is in base: under_cap), 1 - tanh^2 = 4 (w - w^2)
       const float w =
           __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[r] * in) + 1.f);
       s[r] = fmaf(w, -2.f * out, -base[r]);
       if constexpr (FLAT)
         (*flat)[r] = fmaf(-w, w, w);
+    } else {
+      const float t = tanh_of(s[r] * in);
+      s[r] = fmaf(t, out, -base[r]);
+      if constexpr (FLAT)
+        (*flat)[r] = fmaf(-t, t, 1.f) * (1.f / kFlatUp<T>);
     }
   }
 }
@@ -888,13 +898,19 @@ attention_forward_kernel(AttentionCall c) {
           mma<T>(s[rb][kb], a, q[rb][ks]);
       }
 
-    if (c.cap > 0.f) {
+    auto capped = [&](auto is_short) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
-          cap_scores<T, false>(s[rb][kb], c, all4(m[rb] - under_cap<T>(c)),
-                               nullptr);
+          cap_scores<T, decltype(is_short)::value, false>(
+              s[rb][kb], c, all4(m[rb] - under_cap<T>(c)), nullptr);
+    };
+    if (c.cap > 0.f) {
+      if (__builtin_expect(short_cap<T>(c), 1))
+        capped(std::true_type());
+      else
+        capped(std::false_type());
     } else {
       const float in = c.scale * kLog2e;
 #pragma unroll
@@ -1303,13 +1319,19 @@ attention_dq_kernel(AttentionCall c) {
           }
         }
       }
-      if (c.cap > 0.f) {
+      auto capped = [&](auto is_short) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int b = 0; b < S::FB; ++b)
-            cap_scores<T, true>(s[rb][b], c, all4(lse[rb] - under_cap<T>(c)),
-                                &flat[rb][b]);
+            cap_scores<T, decltype(is_short)::value, true>(
+                s[rb][b], c, all4(lse[rb] - under_cap<T>(c)), &flat[rb][b]);
+      };
+      if (c.cap > 0.f) {
+        if (__builtin_expect(short_cap<T>(c), 1))
+          capped(std::true_type());
+        else
+          capped(std::false_type());
       } else {
         const float in = c.scale * kLog2e;
 #pragma unroll
@@ -1536,12 +1558,19 @@ attention_dkv_kernel(AttentionCall c) {
           }
         }
       }
-      if (c.cap > 0.f) {
+      auto capped = [&](auto is_short) {
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
           for (int b = 0; b < S::FB; ++b)
-            cap_scores<T, true>(pr[rb][b], c, lse[b], &flat[rb][b]);
+            cap_scores<T, decltype(is_short)::value, true>(
+                pr[rb][b], c, lse[b], &flat[rb][b]);
+      };
+      if (c.cap > 0.f) {
+        if (__builtin_expect(short_cap<T>(c), 1))
+          capped(std::true_type());
+        else
+          capped(std::false_type());
       } else {
         const float in = c.scale * kLog2e;
 #pragma unroll

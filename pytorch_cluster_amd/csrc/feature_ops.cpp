@@ -11,6 +11,8 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <optional>
 #include <vector>
@@ -108,7 +110,9 @@ struct Attention {
     a.hk = (int32_t)k.size(1);
     a.d = (int32_t)q.size(2);
     a.scale = (float)scale;
-    a.cap = (float)cap;
+    // (fp32 ends at both sides: a cap beyond bends nothing, one below leaves nothing)
+    a.cap = cap > 0.0 ? (float)std::clamp(cap, (double)FLT_MIN, (double)FLT_MAX)
+                      : 0.f;
     return a;
   }
   Tensor workspace(bool backward) const {
