@@ -782,6 +782,13 @@ __device__ __forceinline__ void take_distance(f32x4 (&s)[RB][NB],
 
 // ---- forward ------------------------------------------------------------------
 
+// A row's largest weight is 2^this when what is subtracted is set.  Rounded for the matrix
+// cores, fp16 weights end at 2^-25: with 7 bits above 1 what is lost of a row is below
+// 2^-32 of its largest weight each, with none (2^-25 each) 20,000 keys that far below one
+// other vanish from the products and stay in the sum, 0.06 % of it.  Up to 2^15 fits.
+template <typename T>
+constexpr float kWeightBits = std::is_same<T, _Float16>::value ? 7.f : 0.f;
+
 // Rows of a wave's columns: RB blocks of 16.  WK waves share the same columns and
 // divide every tile among them (few rows); the others own columns of their own.
 //
@@ -789,8 +796,8 @@ __device__ __forceinline__ void take_distance(f32x4 (&s)[RB][NB],
 //
 //   l' = l 2^(m - m') + sum_j 2^(s_j - m')     o' = o 2^(m - m') + sum_j 2^(s_j - m') v_j
 //
-// where m' differs from m only if a score is above m by more than 8: weights are then at
-// most 256, in 32-bit sums, and nearly all tiles skip the scaling.
+// where m' differs from m only if a weight would be above 2^8 (fp16 2^15, see kWeightBits),
+// in 32-bit sums, and nearly all tiles skip the scaling.
 //
 // Bound by the vector unit (see above) where rows are many; by latency where they are
 // few: one cloud of 1,024 rows, 4 heads of 32, fp32, in pieces, 17 us; 32 single queries
@@ -944,19 +951,21 @@ attention_forward_kernel(AttentionCall c) {
           top[rb] = fmaxf(top[rb], s[rb][kb][r]);
     }
 
-    // What is subtracted moves only when a score would be above it by more than 8
-    // (256-fold weights, far from any limit): most tiles leave the sums as they are.
+    // What is subtracted moves only when a weight would be more than 256 times what
+    // the largest was when it was set, far from any limit: most tiles leave the sums
+    // as they are.
     bool move[RB], moves = false;
 #pragma unroll
     for (int rb = 0; rb < RB; ++rb) {
       top[rb] = across_groups_max(top[rb]);
-      move[rb] = top[rb] > 8.f || (!seen[rb] && top[rb] > -__builtin_inff());
+      move[rb] = top[rb] > kWeightBits<T> + 8.f ||
+                 (!seen[rb] && top[rb] > -__builtin_inff());
       moves |= move[rb];
     }
     if (__ballot(moves) != 0) {
 #pragma unroll
       for (int rb = 0; rb < RB; ++rb) {
-        const float by = move[rb] ? top[rb] : 0.f;
+        const float by = move[rb] ? top[rb] - kWeightBits<T> : 0.f;
         const float keep =
             move[rb] && seen[rb] ? __builtin_amdgcn_exp2f(-by) : 1.f;
         seen[rb] |= move[rb];

@@ -28,7 +28,7 @@ TINY = 2.0 ** -126
 def tail(dtype):
     """Of the largest weight of a row: what rounding a weight may take off one
     that is too small for fp16."""
-    return 2.0 ** -25 if dtype == torch.float16 else 0.0
+    return 2.0 ** -32 if dtype == torch.float16 else 0.0
 
 
 def attention_bounds(q, k, v, batch_q=None, batch_k=None, pos_q=None,
