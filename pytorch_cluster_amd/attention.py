@@ -47,7 +47,7 @@ def attention(
             ``u(t) = cap * tanh(t / cap)``.
 
     Returns ``[M, H, C]`` of ``q``'s type.  ``q``, ``k`` and ``v`` get gradients
-    (once: no second derivatives).  Sums are held in 32 bits; the same call
+    (once: second and forward-mode derivatives raise).  Sums are held in 32 bits; the same call
     gives the same bits.  May be captured into a graph.
     """
     return torch.ops.pytorch_cluster_amd.attention(

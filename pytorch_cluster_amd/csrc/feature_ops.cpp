@@ -8,12 +8,14 @@
 // stream.
 #include "ops_common.hpp"
 
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <initializer_list>
 #include <optional>
 #include <vector>
 
@@ -75,6 +77,15 @@ const void *data_or_null(const Tensor &t) {
 void refuse_create_graph(const char *op) {
   TORCH_CHECK(!at::GradMode::is_enabled(), op,
               " cannot be differentiated twice (create_graph=True)");
+}
+
+// So would a forward-mode derivative, where no input wants a gradient.
+void refuse_tangents(const char *op, std::initializer_list<Tensor> tensors) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    return;
+  for (const Tensor &t : tensors)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), op,
+                " has no forward-mode derivative");
 }
 
 // ---- attention ------------------------------------------------------------------
@@ -277,6 +288,7 @@ Tensor attention(const Tensor &q, const Tensor &k, const Tensor &v,
   TORCH_CHECK(std::isfinite(factor), "attention: scale has to be finite");
   TORCH_CHECK(std::isfinite(cap) && cap >= 0.0,
               "attention: cap has to be finite and not negative");
+  refuse_tangents("attention", {q, k, v, at_q, at_k, slopes});
 
   PCA_CHECK_GPU(q);
   for (const Tensor &t :
@@ -470,6 +482,8 @@ std::vector<Tensor> norm_rotate(const Tensor &q, const Maybe &k,
                 "norm_rotate: weight_q and weight_k have to be of one type");
   TORCH_CHECK(std::isfinite(eps) && eps >= 0.0,
               "norm_rotate: eps has to be finite and not negative");
+  refuse_tangents("norm_rotate", {q, or_none(k), pos, freq, or_none(weight_q),
+                                  or_none(weight_k)});
 
   PCA_CHECK_GPU(q);
   for (const Tensor &t :
@@ -563,6 +577,7 @@ Tensor lookup(const Tensor &weight, const Tensor &index, double scale) {
               "lookup: index has to be int64 or int32, got ",
               index.scalar_type());
   TORCH_CHECK(std::isfinite(scale), "lookup: scale has to be finite");
+  refuse_tangents("lookup", {weight});
   PCA_CHECK_GPU(weight);
   TORCH_CHECK(index.device() == weight.device(), "lookup: tensors on ",
               weight.device(), " and ", index.device());

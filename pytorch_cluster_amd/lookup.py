@@ -19,8 +19,8 @@ def lookup(weight: torch.Tensor, index: torch.Tensor,
             output row is zeros and it adds to no gradient.
         scale: factor of the rows.
 
-    Returns ``[*index.shape, C]``.  ``weight`` gets a gradient (once), summed in
-    32 bits from the entries in the order of their rows: the same call gives
-    the same bits.
+    Returns ``[*index.shape, C]``.  ``weight`` gets a gradient (once: second
+    and forward-mode derivatives raise), summed in 32 bits from the entries in
+    the order of their rows: the same call gives the same bits.
     """
     return torch.ops.pytorch_cluster_amd.lookup(weight, index, scale)

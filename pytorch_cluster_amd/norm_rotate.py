@@ -34,7 +34,8 @@ def norm_rotate(
         eps: added to the mean square.
 
     Returns ``q`` and ``k`` (or ``None``) normed and turned.  ``q``, ``k`` and
-    the weights get gradients (once).
+    the weights get gradients (once: second and forward-mode derivatives
+    raise).
     """
     outs = torch.ops.pytorch_cluster_amd.norm_rotate(q, k, pos, freq, weight_q,
                                                      weight_k, eps)

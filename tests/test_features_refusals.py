@@ -1,0 +1,42 @@
+"""What attention, norm_rotate and lookup refuse beyond shapes and types (no GPU):
+forward-mode derivatives.
+"""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+import pytorch_cluster_amd as pca
+
+
+def arguments(op):
+    rows = torch.zeros(6, 4, 8)
+    if op == "attention":
+        return dict(q=rows, k=rows.clone(), v=rows.clone(),
+                    pos_q=torch.zeros(6, 3), pos_k=torch.zeros(6, 3),
+                    slope=torch.zeros(4))
+    if op == "norm_rotate":
+        return dict(q=rows, k=rows.clone(), pos=torch.zeros(6, 3),
+                    freq=torch.zeros(3, 4), weight_q=torch.ones(8),
+                    weight_k=torch.ones(8))
+    return dict(weight=torch.zeros(6, 4), index=torch.zeros(3, dtype=torch.long))
+
+
+@pytest.mark.parametrize("op,name", [
+    (op, n) for op in ("attention", "norm_rotate", "lookup")
+    for n, t in arguments(op).items() if t.is_floating_point()])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(op, name, grad):
+    args = arguments(op)
+    differentiable = name in ("q", "k", "v", "weight_q", "weight_k", "weight")
+    with fwd.dual_level():
+        primal = args[name].clone().requires_grad_(grad and differentiable)
+        args[name] = fwd.make_dual(primal, torch.ones_like(primal))
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            getattr(pca, op)(**args)
+        with torch.no_grad():
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                getattr(pca, op)(**args)
+    # (without a tangent: as far as the device)
+    with fwd.dual_level():
+        with pytest.raises(RuntimeError, match="must be CUDA tensor"):
+            getattr(pca, op)(**arguments(op))
