@@ -123,7 +123,7 @@ int norm_rotate_call(const pca_norm_rotate_args *a, pca::NormRotateCall &c) {
   if (a->rows < 0 || a->rows > kMost || a->hq < 1 || a->hk < 0 ||
       a->hq > 65535 || a->hk > 65535 || a->d < 1 ||
       a->d > PCA_NORM_ROTATE_MAX_D || a->axes < 1 || a->axes > 3 ||
-      a->rotated < 0 || 2 * a->rotated > a->d)
+      a->rotated < 0 || a->rotated > a->d / 2)
     return pca::fail(PCA_ERR_INVALID_ARGUMENT,
                      "norm_rotate: sizes out of range (%lld rows, %d + %d heads "
                      "of %d, %d axes, %d pairs)",

@@ -1,11 +1,16 @@
 """What attention, norm_rotate and lookup refuse beyond shapes and types (no GPU):
-forward-mode derivatives.
+forward-mode derivatives, numbers at the ends of their types in the C ABI.
 """
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
 import pytorch_cluster_amd as pca
+from pytorch_cluster_amd import _native
+
+AT = 1 << 20  # (an address that is never used)
 
 
 def arguments(op):
@@ -40,3 +45,18 @@ def test_forward_mode_is_refused(op, name, grad):
     with fwd.dual_level():
         with pytest.raises(RuntimeError, match="must be CUDA tensor"):
             getattr(pca, op)(**arguments(op))
+
+
+@pytest.mark.parametrize("rotated", [9, 2 ** 30, 2 ** 30 + 5, 2 ** 31 - 1, -1,
+                                     -2 ** 30, -2 ** 31])
+def test_pairs_that_do_not_fit_a_head(rotated):
+    # (twice 2^30 does not fit 32 bits)
+    args = _native.NormRotateArgs(q=AT, rows=10, hq=2, hk=0, d=16, axes=2,
+                                  rotated=rotated, pos=AT, freq=AT, dtype=3,
+                                  weight_dtype=0, eps=1e-6)
+    lib = _native.capi
+    assert lib.pca_norm_rotate_forward(ctypes.byref(args), AT, None, None) == -1
+    size = lib.pca_norm_rotate_workspace_bytes(10, 16)
+    assert lib.pca_norm_rotate_backward(
+        ctypes.byref(args), AT, 32, 16, None, 0, 0, AT, None, None, None, AT,
+        size, None) == -1
