@@ -125,7 +125,7 @@ int pca_norm_rotate_backward(const pca_norm_rotate_args *args,
 /*
  * out[e] = scale table[index[e]]; zeros where the index lies outside
  * [0, table_rows).  index: int32 or int64 (index_bytes 4 or 8).  table:
- * [table_rows, width] dense, out: [entries, width] dense.
+ * [table_rows, width] dense, out: [entries, width] dense.  scale is finite.
  */
 int pca_lookup(const void *table, const void *index, int32_t index_bytes,
                int64_t table_rows, int64_t entries, int64_t width, float scale,

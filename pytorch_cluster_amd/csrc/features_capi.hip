@@ -176,6 +176,8 @@ int lookup_call(const void *rows, const void *index, int32_t index_bytes,
   if (!on16(rows) || !on16(out))
     return pca::fail(PCA_ERR_INVALID_ARGUMENT,
                      "lookup: tensors have to start on 16 bytes");
+  if (!std::isfinite(scale))
+    return pca::fail(PCA_ERR_INVALID_ARGUMENT, "lookup: scale has to be finite");
   c.rows = rows;
   c.index = index;
   c.wide_index = index_bytes == 8;

@@ -60,3 +60,14 @@ def test_pairs_that_do_not_fit_a_head(rotated):
     assert lib.pca_norm_rotate_backward(
         ctypes.byref(args), AT, 32, 16, None, 0, 0, AT, None, None, None, AT,
         size, None) == -1
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_factors_of_rows_that_are_no_numbers(scale):
+    # (times a component of zero: NaN)
+    lib = _native.capi
+    assert lib.pca_lookup(AT, AT, 8, 10, 5, 4, scale, 0, AT, None) == -1
+    assert b"finite" in lib.pca_last_error()
+    size = lib.pca_lookup_grad_workspace_bytes(10, 5, 4)
+    assert lib.pca_lookup_grad(AT, AT, 8, 10, 5, 4, scale, 0, AT, AT, size,
+                               None) == -1
