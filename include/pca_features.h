@@ -58,7 +58,8 @@ typedef struct pca_attention_args {
   const float *slope;               /* [hq], or NULL: no bias                 */
   int32_t axes;                     /* 1 .. 3                                 */
   int32_t dtype;
-  int64_t nq, nk;                   /* nq * hq / hk, nk < 2^31 - 1,024        */
+  int64_t nq, nk;                   /* nq * hq / hk and nk, each rounded up   */
+                                    /* to 64, times hk: below 2^30            */
   int32_t hq, hk, d;                /* hq a multiple of hk, d <= 128          */
   float scale;
   float cap;                        /* 0: none                                */

@@ -1725,7 +1725,7 @@ hipError_t launch(const AttentionCall &c, int pass, int rows,
   const int64_t grid = (owned + rows - 1) / rows * c.hk * c.splits;
   if (grid <= 0)
     return hipSuccess;
-  if (grid * kThreads > UINT32_MAX) // (what a launch can number)
+  if (grid * kThreads > UINT32_MAX) // (what a launch can number; checked before)
     return hipErrorInvalidValue;
   const dim3 g((unsigned)grid), b(kThreads);
 #define PCA_LAUNCH(kernel, most)                                               \

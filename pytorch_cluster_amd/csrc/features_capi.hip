@@ -14,6 +14,7 @@ namespace {
 constexpr int64_t kMost = 2147483646; // rows, entries
 // Rows of attention's sides (times heads of a group): with room for a tile behind them.
 constexpr int64_t kMostOwned = kMost - 1024;
+constexpr int64_t kMostGroups = UINT32_MAX / 256;
 
 bool type_ok(int dtype) {
   return dtype == PCA_F32 || dtype == PCA_F16 || dtype == PCA_BF16;
@@ -59,8 +60,10 @@ bool attention_sizes_ok(int64_t nq, int64_t nk, int64_t hq, int64_t hk,
          hq % hk == 0 && hq <= 65535 && nq <= kMostOwned / (hq / hk) &&
          d >= 1 &&
          d <= PCA_ATTENTION_MAX_D &&
-         // (workgroups of 16 owned rows, numbered by an int)
-         (nq / 16 + 1) * hq < kMost && (nk / 16 + 1) * hk < kMost;
+         // (workgroups of 64 owned rows or more, 256 threads, that one launch numbers;
+         // of 16 rows where they are at most 256)
+         (nq * (hq / hk) + 63) / 64 * hk <= kMostGroups &&
+         (nk + 63) / 64 * hk <= kMostGroups;
 }
 
 int attention_call(const pca_attention_args *a, pca::AttentionCall &c) {

@@ -71,3 +71,26 @@ def test_factors_of_rows_that_are_no_numbers(scale):
     size = lib.pca_lookup_grad_workspace_bytes(10, 5, 4)
     assert lib.pca_lookup_grad(AT, AT, 8, 10, 5, 4, scale, 0, AT, AT, size,
                                None) == -1
+
+
+@pytest.mark.parametrize("heads", [1, 2, 7])
+@pytest.mark.parametrize("side", ["nq", "nk"])
+def test_rows_that_one_launch_cannot_take(heads, side):
+    # 64 rows of a key head a workgroup of 256, 2^32 threads in a launch
+    most = (2 ** 24 - 1) // heads * 64
+
+    def sizes(n):
+        return (n, 5) if side == "nq" else (5, n)
+
+    def workspace(n, backward):
+        return _native.capi.pca_attention_workspace_bytes(
+            *sizes(n), heads, heads, 1, backward)
+    for backward in (0, 1):
+        assert workspace(most, backward) > 0
+        assert workspace(most + 1, backward) == 0
+    nq, nk = sizes(most + 1)
+    args = _native.AttentionArgs(q=AT, k=AT, v=AT, nq=nq, nk=nk, hq=heads,
+                                 hk=heads, d=1, dtype=0, scale=1.0, cap=0.0)
+    assert _native.capi.pca_attention_forward(
+        ctypes.byref(args), AT, None, None, AT, 1 << 40, None) == -1
+    assert b"out of range" in _native.capi.pca_last_error()
