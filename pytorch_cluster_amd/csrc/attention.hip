@@ -311,7 +311,7 @@ AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
   auto groups = [&](int rows) { return (owned + rows - 1) / rows * hk; };
   AttentionPlan p;
   p.rows = most_rows(pass, size, d);
-  if (d <= 32 || (d <= 64 && pass != 2 && size == 2) || groups(p.rows) < 512)
+  if (groups(p.rows) < 512)
     p.rows = 64;
   if (owned <= 256)
     p.rows = kFewRows;

@@ -83,10 +83,14 @@ PCA_ATTENTION_DECLARE(bf16);
 // many.  Two blocks of 16 columns per wave share every left operand; where the sums of
 // both do not fit the registers of two waves per SIMD it is one.  Heads of 128, 128 rows
 // against 64: bf16 forward 291 us against 404 (with bias and cap 488, 549), dq 680 - 1,036
-// against 632 - 646; fp32 forward 726 against 587.
+// against 632 - 646; fp32 forward 726 against 587.  Narrow heads have few sums, and four
+// waves per SIMD of one block cover more (attention_plan has what was measured).
 constexpr int kFewRows = 16;
 constexpr int most_rows(int pass, int size, int width) {
-  return width > 64 && (pass > 0 || size == 4) ? 64 : 128;
+  return width <= 32 || (width <= 64 && pass != 2 && size == 2) ||
+                 (width > 64 && (pass > 0 || size == 4))
+             ? 64
+             : 128;
 }
 
 // Looped rows of a piece, at least: four tiles of fp32 rows, eight of 16-bit ones.  With
