@@ -42,3 +42,40 @@ def test_every_kernel_that_is_built_is_taken():
                     rows, _ = plan(kind, n, n, 8, 8, size, w)
                     taken.add((kind, name, w) + kernel[rows])
     assert built == taken
+
+
+def many_rows():
+    """Sizes of 64 examples, of none to 400 rows, in which rows of several examples
+    share a tile: at 8 key heads enough for 128 rows a workgroup."""
+    sizes = [(37 * i * i + 11 * i) % 401 for i in range(64)]
+    sizes[5], sizes[6], sizes[7] = 1, 0, 2
+    return sizes
+
+
+# Heads of which some pass has kernels of 128 rows, and what is cut into pieces: type
+# (size), width, pass.
+WIDE_TILES = [(2, 33, "dkv"), (2, 48, "dkv"), (2, 63, "dkv"), (2, 64, "dkv"),
+              (2, 65, "forward"), (2, 96, "forward"), (2, 100, "forward"),
+              (2, 127, "forward"), (2, 128, "forward")] + [
+    (4, d, p) for d in (33, 48, 57, 64) for p in PASSES]
+
+
+@pytest.mark.parametrize("size,d,kind", WIDE_TILES)
+@pytest.mark.parametrize("heads", [8, 16])
+def test_many_rows_take_tiles_of_128(size, d, kind, heads):
+    n = sum(many_rows())
+    assert plan(kind, n, n, heads, 8, size, d) == (128, 1)
+
+
+# Rows and heads whose looped side is cut into pieces of tiles of 16 and of 64 rows.
+CUT = [(1100, 2), (100, 1)]
+
+
+@pytest.mark.parametrize("size", [2, 4])
+@pytest.mark.parametrize("d", [5, 31, 65, 127])
+@pytest.mark.parametrize("kind", PASSES)
+@pytest.mark.parametrize("owned,heads", CUT)
+def test_few_rows_are_cut_into_pieces(size, d, kind, owned, heads):
+    sides = (owned, 2300) if kind != "dkv" else (2300, owned)
+    rows, pieces = plan(kind, *sides, heads, heads, size, d)
+    assert rows == (16 if owned <= 256 else 64) and pieces > 1
