@@ -62,7 +62,7 @@ typedef struct pca_attention_args {
                                     /* to 64, times hk: below 2^30            */
   int32_t hq, hk, d;                /* hq a multiple of hk, d <= 128          */
   float scale;
-  float cap;                        /* 0: none                                */
+  float cap;                        /* 0: none; above 2^127: 2^127            */
 } pca_attention_args;
 
 /* Scratch of the forward (backward = 0) or the backward call (1); 0: sizes not
@@ -92,7 +92,8 @@ int pca_attention_backward(const pca_attention_args *args, const void *out,
  *   out_c = y_c cos a_c - y_{c + rotated} sin a_c
  *   out_{c + rotated} = y_{c + rotated} cos a_c + y_c sin a_c
  *
- * and y itself from element 2 rotated on.
+ * and y itself from element 2 rotated on.  The mean is formed in 32 bits: x^2
+ * has to stay in their range.
  */
 typedef struct pca_norm_rotate_args {
   const void *q, *k;                /* [rows, hq, d], [rows, hk, d]           */
@@ -126,7 +127,8 @@ int pca_norm_rotate_backward(const pca_norm_rotate_args *args,
 /*
  * out[e] = scale table[index[e]]; zeros where the index lies outside
  * [0, table_rows).  index: int32 or int64 (index_bytes 4 or 8).  table:
- * [table_rows, width] dense, out: [entries, width] dense.  scale is finite.
+ * [table_rows, width] dense, out: [entries, width] dense.  scale is finite;
+ * rows and entries are below 2^31 - 1, width at most 2^20.
  */
 int pca_lookup(const void *table, const void *index, int32_t index_bytes,
                int64_t table_rows, int64_t entries, int64_t width, float scale,

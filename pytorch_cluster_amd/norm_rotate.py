@@ -31,7 +31,9 @@ def norm_rotate(
         weight_q: ``[C]`` gain of ``q`` (default ones), of ``q``'s type or
             float32.
         weight_k: the same for ``k``.
-        eps: added to the mean square.
+        eps: added to the mean square, which is formed in 32 bits: components
+            beyond ``1e18``, or without ``eps`` all below ``1e-18``, leave its
+            range.
 
     Returns ``q`` and ``k`` (or ``None``) normed and turned.  ``q``, ``k`` and
     the weights get gradients (once: second and forward-mode derivatives
