@@ -44,11 +44,18 @@ def attention(
             the score; no gradient.
         scale: factor of the products (default ``C ** -0.5``).
         cap: if positive, products are bounded before the bias is added:
-            ``u(t) = cap * tanh(t / cap)``.
+            ``u(t) = cap * tanh(t / cap)``; any size (above ``2 ** 127`` that
+            counts).
 
     Returns ``[M, H, C]`` of ``q``'s type.  ``q``, ``k`` and ``v`` get gradients
-    (once: second and forward-mode derivatives raise).  Sums are held in 32 bits; the same call
-    gives the same bits.  May be captured into a graph.
+    (once: second and forward-mode derivatives raise).
+
+    Scores, softmax statistics and sums are held in 32 bits.  With 16-bit rows
+    the weights, and in the backward pass the scores' gradients, are rounded
+    once to that type for the matrix cores; float32 rows round nothing below
+    32 bits.  The same call gives the same bits.  May be captured into a graph;
+    as with any operator of torch, a backward pass is captured while no eager
+    graph of the same leaves is alive.
     """
     return torch.ops.pytorch_cluster_amd.attention(
         q, k, v, batch_q, batch_k, pos_q, pos_k, slope, scale, cap)

@@ -302,7 +302,8 @@ int element_size(int dtype) { return dtype == 0 ? 4 : 2; }
 // 1,024 workgroups on pieces lose (clouds, one and two: 384, 497).  With 16 rows a
 // workgroup 512 workgroups' worth (32 queries, 16 to 128 pieces: 58, 60, 71, 97).  How many
 // of the pieces a tile of rows uses goes by the length of its own examples
-// (pieces_in_use).
+// (pieces_in_use).  Rows are counted, which is right for long examples; many short ones
+// are a longer chain of tiles than their rows say.
 AttentionPlan attention_plan(int pass, int64_t nq, int64_t nk, int hq, int hk,
                              int size, int d) {
   const int64_t rows_q = nq * (hq / hk);

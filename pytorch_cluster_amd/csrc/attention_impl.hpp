@@ -42,17 +42,22 @@
 //
 // What bounds them (one MI355X; 16 clouds of 1,024 rows, 8 heads of 64, bf16, positions
 // on three axes): the vector unit.  64 pairs of rows cost 17 - 19 vector instructions
-// (distance 7; exponential and square root at a quarter of the rate).  Forward 104 us, the
-// vector unit busy for 81 % of the cycles and the matrix cores for 17; dq 120 us, 67 and
-// 21 %; dk and dv 151 us, 54 and 21 %, with two waves per SIMD, which no longer cover
-// each other's products, exchanges and barriers.  Without bias and cap the forward
-// reaches 938 TFLOP/s with heads of 128 (4 examples of 4,096 rows, 8 heads, bf16: 293
-// us) and 681 with heads of 64, forward and backward 668 and 631 (a product of 8,192^3:
-// 1,261); fp32, where the matrix cores are busy for half of the cycles, 112 - 116 of 153.
+// (exponential and square root at a quarter of the rate); 7 of them and the square root are
+// the distance, which is the same for all heads and formed again for each of them, in each
+// of the three kernels.  Forward 104 us, the vector unit busy for 81 % of the cycles and the
+// matrix cores for 16; dq 120 us, 69 and 21 %; dk and dv 156 us, 53 and 21 %, with two
+// waves per SIMD, which no longer cover each other's products, exchanges and barriers.
+// Without bias and cap a forward call reaches 912 TFLOP/s with heads of 128 (4 examples
+// of 4,096 rows, 8 heads, bf16: 301 us) and 687 with heads of 64, forward and backward 694
+// and 639 (a product of 8,192^3: 1,261); fp32, where the matrix cores are busy for half of
+// the cycles, 117 - 122 of 153, and 95 with the backward pass.
 //
 // Tiles come by loads that bypass the registers (request16), one tile ahead: with loads
 // into registers and stores to LDS 4 examples of 4,096 rows with everything on took 1,312
-// / 1,375 / 1,833 us instead of 576 / 680 / 964 (now 485 / 654 / 855).
+// / 1,375 / 1,833 us instead of 576 / 680 / 964 (now 493 / 643 / 858).
+//
+// Exponentials, reciprocals, square roots and logarithms are the vector unit's own, off by
+// a step of fp32; results below 2^-126 are zeros.
 #pragma once
 
 #include "attention.hpp"
@@ -149,7 +154,9 @@ __device__ __forceinline__ u32x4 load_piece(const HeadRows &x, int64_t row,
 static __device__ const uint32_t kZeros[4] = {0, 0, 0, 0};
 
 // Loads that go from memory to LDS without registers: lane l's 16 (4) bytes to `lds` +
-// 16 l (4 l).  Nothing waits for them but arrive().
+// 16 l (4 l).  Nothing waits for them but arrive().  (m0 is written and used inside one
+// statement: the compiler keeps nothing in it between statements, and has it reserved, so
+// that it cannot be named as clobbered.)
 __device__ __forceinline__ void request16(const void *from, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\t"
                "s_nop 0\n\t"
@@ -667,7 +674,9 @@ constexpr float kFlatUp = std::is_same<T, float>::value ? 1.f : 4.f;
 // Up to which cap 16-bit rows take the short form, cap (1 - 2 w) with the cap itself in
 // `base`: an exponential and a reciprocal, but what it rounds is as large as the cap, so
 // a score is off by 1.7e-7 cap: 2e-5 here, a 24th of what rounding a weight to fp16 takes
-// off.  Beyond, and in fp32, a score is as exact as its own size (tanh_of).
+// off.  Beyond, and in fp32, a score is as exact as its own size (tanh_of): 16,384 rows of
+// 8 heads of 128 in four examples, bf16, forward 509 us instead of 361, with the backward
+// pass 1,999 instead of 1,595.
 constexpr float kShortCap = 128.f;
 template <typename T>
 __device__ __forceinline__ bool short_cap(const AttentionCall &c) {
@@ -1178,8 +1187,8 @@ store_columns(const Sums<T, DP, RB> &acc, int rb, void *out, float *part,
 // Scores are formed again (P = 2^(s - lse): no memory for them), three products a pair.
 // -delta is what the product with v starts from.  A step is as many rows as the matrix
 // instruction's contraction, so that scores and dP of a step alone hold registers.  4 x
-// 4,096 rows, 8 heads of 128, bf16, bias and cap: 654 us, 630 TFLOP/s of its three
-// products; vector unit 49 %, matrix cores 28 %, LDS 30 % of the cycles at two waves per
+// 4,096 rows, 8 heads of 128, bf16, bias and cap: 643 us, 641 TFLOP/s of its three
+// products; vector unit 50 %, matrix cores 28 %, LDS 31 % of the cycles at two waves per
 // SIMD.  One block of columns per wave, since two spill (680 -
 // 1,036 us).
 template <typename T, int DP, int RB, int WK>
@@ -1442,7 +1451,7 @@ attention_dq_kernel(AttentionCall c) {
 //
 // Four products a pair.  A row's numbers (position, slope, lse, delta) come with its
 // tile.  P goes to dv's product, dT to dk's, both rounded for the matrix cores.  The
-// call above: 855 us, 643 TFLOP/s of its four products; vector unit 43 %, matrix cores
+// call above: 858 us, 641 TFLOP/s of its four products; vector unit 42 %, matrix cores
 // 28 %, LDS 35 %.
 template <typename T, int DP, int RB, int WK>
 __global__ __launch_bounds__(kThreads, (waves_wanted<T, DP, RB, WK>())) void

@@ -14,7 +14,8 @@
 // the workspace, and the chunk where a run starts adds up its parts.  The same call
 // gives the same bits.
 //
-// Bound by memory.  1,310,720 entries of 64 fp32 components in a table of 65,536 rows:
+// The forward pass is bound by memory; of the gradient 40 % is the sort, mostly ranks in
+// LDS and six launches, and the sums are memory's.  1,310,720 entries of 64 fp32 components in a table of 65,536 rows:
 // forward 96 us = 3.6 TB/s of output and indices (the table comes from the caches, whose
 // reads of single rows are what keeps it from the copy's 5.0); gradient: digits 16 + 9
 // + 39 us (count, scan, scatter of two passes), sums 81 us = 4.1 TB/s, joins 9.5 us.
